@@ -29,7 +29,7 @@ def private_arrays(src: Path) -> list[tuple[str, str]]:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     with tempfile.TemporaryDirectory() as d:
         out = Path(d) / "k.ll"
-        subprocess.run([hipcc, "-O3", "-std=c++17", "--offload-arch=gfx950", "-fno-fast-math", "-I", str(ROOT / "csrc"),
+        subprocess.run([hipcc, "-O3", "-std=c++17", "--offload-arch=gfx950", "-fno-fast-math", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", str(ROOT / "csrc"),
                         "--cuda-device-only", "-S", "-emit-llvm", "-o", str(out), str(src)],
                        check=True, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
         found, fn = [], "?"

@@ -36,7 +36,7 @@ ALLOWED = {
 
 def spills(src: Path) -> list[tuple[str, int]]:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    r = subprocess.run([hipcc, "-O3", "-std=c++17", "--offload-arch=gfx950", "-fno-fast-math", "-I", str(ROOT / "csrc"),
+    r = subprocess.run([hipcc, "-O3", "-std=c++17", "--offload-arch=gfx950", "-fno-fast-math", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", str(ROOT / "csrc"),
                         "-I", str(ROOT / "csrc" / "kernels"), "--cuda-device-only", "-Rpass-analysis=kernel-resource-usage",
                         "-c", "-o", os.devnull, str(src)], capture_output=True, text=True)
     if r.returncode != 0:
