@@ -13,6 +13,7 @@
 #include "comm/async_shards.h"
 #include "comm/link_probe.h"
 #include "kernels/conv.h"
+#include "kernels/linear.h"
 #include "kernels/ops.h"
 #include "runtime/program.h"
 
@@ -479,6 +480,50 @@ PYBIND11_MODULE(_hip, m) {
     V(M); V(N); V(K); V(lda); V(ldb); V(ldc); V(trans_a); V(trans_b); V(relu); V(accumulate); V(variant); V(splits);
     gemm_f32(a, as_stream(stream));
   });
+  // Dense layers: positional, since a single-row call costs no more than its Python call does. An address is 0 for a
+  // tensor that is left out; the workspace query takes the same arguments.
+  {
+    auto fwd = [](int kind, int M, int N, int K, int trans_w, int act, uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t bias,
+                  uint64_t res, long long ldr, uint64_t y, long long ldy, uint64_t pre, long long ldp) {
+      LinearArgs a{};
+      a.kind = kind; a.M = M; a.N = N; a.K = K; a.trans_w = trans_w; a.act = act;
+      a.x = reinterpret_cast<const void*>(x); a.ldx = ldx; a.w = reinterpret_cast<const void*>(w); a.ldw = ldw;
+      a.bias = reinterpret_cast<const void*>(bias); a.res = reinterpret_cast<const void*>(res); a.ldr = ldr;
+      a.y = reinterpret_cast<void*>(y); a.ldy = ldy; a.pre = reinterpret_cast<void*>(pre); a.ldp = ldp;
+      return a;
+    };
+    m.def("linear_workspace", [fwd](int kind, int M, int N, int K, int trans_w, int act, uint64_t x, long long ldx, uint64_t w, long long ldw,
+                                    uint64_t bias, uint64_t res, long long ldr, uint64_t y, long long ldy, uint64_t pre, long long ldp) {
+      return linear_workspace(fwd(kind, M, N, K, trans_w, act, x, ldx, w, ldw, bias, res, ldr, y, ldy, pre, ldp));
+    });
+    m.def("linear", [fwd](int kind, int M, int N, int K, int trans_w, int act, uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t bias,
+                          uint64_t res, long long ldr, uint64_t y, long long ldy, uint64_t pre, long long ldp, uint64_t ws, size_t ws_bytes,
+                          uint64_t stream) {
+      linear(fwd(kind, M, N, K, trans_w, act, x, ldx, w, ldw, bias, res, ldr, y, ldy, pre, ldp), reinterpret_cast<void*>(ws), ws_bytes,
+             as_stream(stream));
+    });
+    auto bwd = [](int kind, int M, int N, int K, int trans_w, int act, int accumulate, uint64_t dy, long long lddy, uint64_t pre, long long ldp,
+                  uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t dx, long long lddx, uint64_t dw, long long lddw, uint64_t db) {
+      LinearBwdArgs a{};
+      a.kind = kind; a.M = M; a.N = N; a.K = K; a.trans_w = trans_w; a.act = act; a.accumulate = accumulate;
+      a.dy = reinterpret_cast<const void*>(dy); a.lddy = lddy; a.pre = reinterpret_cast<const void*>(pre); a.ldp = ldp;
+      a.x = reinterpret_cast<const void*>(x); a.ldx = ldx; a.w = reinterpret_cast<const void*>(w); a.ldw = ldw;
+      a.dx = reinterpret_cast<void*>(dx); a.lddx = lddx; a.dw = reinterpret_cast<void*>(dw); a.lddw = lddw;
+      a.db = reinterpret_cast<void*>(db);
+      return a;
+    };
+    m.def("linear_bwd_workspace", [bwd](int kind, int M, int N, int K, int trans_w, int act, int accumulate, uint64_t dy, long long lddy, uint64_t pre,
+                                        long long ldp, uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t dx, long long lddx, uint64_t dw,
+                                        long long lddw, uint64_t db) {
+      return linear_bwd_workspace(bwd(kind, M, N, K, trans_w, act, accumulate, dy, lddy, pre, ldp, x, ldx, w, ldw, dx, lddx, dw, lddw, db));
+    });
+    m.def("linear_bwd", [bwd](int kind, int M, int N, int K, int trans_w, int act, int accumulate, uint64_t dy, long long lddy, uint64_t pre,
+                              long long ldp, uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t dx, long long lddx, uint64_t dw,
+                              long long lddw, uint64_t db, uint64_t ws, size_t ws_bytes, uint64_t stream) {
+      linear_bwd(bwd(kind, M, N, K, trans_w, act, accumulate, dy, lddy, pre, ldp, x, ldx, w, ldw, dx, lddx, dw, lddw, db),
+                 reinterpret_cast<void*>(ws), ws_bytes, as_stream(stream));
+    });
+  }
   m.def("col_sum", [](const py::dict& d, uint64_t stream) {
     ColSumArgs a{};
     P(x, const float); P(out, float); V(n_rows); V(C); P(relu_of, const float); P(masked, float);
@@ -510,6 +555,7 @@ PYBIND11_MODULE(_hip, m) {
   });
 
   // ---------------------------------------------------------------- step programs
+  m.def("recording", []() { return current_recorder() != nullptr; });
   py::class_<Program>(m, "Program")
       .def(py::init<>())
       .def("begin_record", [](Program& p) {

@@ -1,0 +1,174 @@
+// Dense layers y = act(x W + b) + residual in fp32, bf16 and fp16, and their gradients: the host side, which
+// picks a product kernel (linear_tile.h) and lays out the workspace.
+//
+// Per output element the forward pass costs 2 K flops and the epilogue rides in the product's registers: bias, the
+// stored pre-activation, the activation and the residual cost their own bytes and no launch. The backward pass
+// is one pass over dy and the pre-activation (dz and the column sums) and two products.
+#include "linear_tile.h"
+
+namespace dtf {
+namespace {
+
+constexpr size_t kMaxPartialBytes = 256ull << 20;   // partial sums of a split product
+
+const LinLaunch& lin_launch(int kind) {
+  switch (kind) {
+    case MM_F32: return lin_launch_f32();
+    case MM_BF16: return lin_launch_bf16();
+    case MM_F16: return lin_launch_f16();
+    default: throw std::runtime_error("linear: unknown element type");
+  }
+}
+int elem_bytes(int kind) { return kind == MM_F32 ? 4 : 2; }
+bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+size_t round_up(size_t v) { return (v + 255) & ~(size_t)255; }
+
+struct Plan {
+  int variant, splits, k_per_split, gx, gy;
+  long long N4;
+  size_t bytes;
+};
+Plan plan_of(const MmProduct& p) {
+  Plan l{};
+  l.variant = LIN_REGS_128;
+  const int bm = kLinVariants[l.variant].bm, bn = kLinVariants[l.variant].bn;
+  const int kb = 128 / elem_bytes(p.kind);
+  l.gx = ceil_div(p.N, bn);
+  l.gy = ceil_div(p.M, bm);
+  l.N4 = ((long long)p.N + 3) / 4 * 4;
+  // Few tiles and a long k: several workgroups share a tile's k, at least four stages each, until every CU has one.
+  const long long tiles = (long long)l.gx * l.gy;
+  const int stages = ceil_div(p.K, kb);
+  int splits = 1;
+  while (tiles * splits * 2 <= 512 && stages >= splits * 8 && (size_t)p.M * l.N4 * splits * 8 <= kMaxPartialBytes) splits *= 2;
+  const int per = ceil_div(stages, splits) * kb;
+  l.splits = p.K > 0 ? ceil_div(p.K, per) : 1;
+  l.k_per_split = p.K > 0 ? per : kb;
+  l.bytes = l.splits > 1 ? round_up((size_t)l.splits * p.M * l.N4 * sizeof(float)) : 0;
+  return l;
+}
+
+void check_ws(const char* what, size_t need, const void* ws, size_t have) {
+  if (need > have || (need && (!ws || !aligned_to(ws, 16)))) throw std::runtime_error(std::string(what) + ": workspace too small or unaligned");
+}
+
+// rows of a dz block: enough blocks to fill the card, at least 16 rows each
+int dz_rows(int M, int N) {
+  if (M <= 0 || N <= 0) return 16;
+  const int col_blocks = ceil_div(N, 256);
+  int blocks = ceil_div(1024, col_blocks);
+  if (blocks > 64) blocks = 64;
+  int rows = ceil_div(M, blocks);
+  return rows < 16 ? 16 : rows;
+}
+
+}  // namespace
+
+size_t mm_product_workspace(const MmProduct& p) { return p.M > 0 && p.N > 0 ? plan_of(p).bytes : 0; }
+
+void mm_product(const MmProduct& p, void* ws, size_t ws_bytes, hipStream_t stream) {
+  if (p.M <= 0 || p.N <= 0) return;
+  const Plan l = plan_of(p);
+  check_ws("linear", l.bytes, ws, ws_bytes);
+  if ((long long)l.gx * l.gy * l.splits > 0x3fffffff) throw std::runtime_error("linear: the product has too many tiles");
+  LinTileArgs a{};
+  a.p = p;
+  a.partial = reinterpret_cast<float*>(ws);
+  a.N4 = l.N4;
+  a.k_per_split = l.k_per_split;
+  a.gx = l.gx; a.gy = l.gy; a.splits = l.splits; a.total = l.gx * l.gy * l.splits;
+  const int v4 = 4 * elem_bytes(p.kind);
+  a.vec = !(p.N & 3) && !(p.ldc & 3) && aligned_to(p.c, v4) && (!p.bias || aligned_to(p.bias, v4)) &&
+          (!p.res || (!(p.ldr & 3) && aligned_to(p.res, v4))) && (!p.pre || (!(p.ldp & 3) && aligned_to(p.pre, v4)));
+  const LinLaunch& f = lin_launch(p.kind);
+  f.tile(a, l.variant, stream);
+  if (l.splits > 1) f.join(a, stream);
+}
+
+namespace {
+MmProduct forward_of(const LinearArgs& a) {
+  MmProduct p{};
+  p.kind = a.kind;
+  p.kc_a = 1; p.kc_b = a.trans_w;
+  p.M = a.M; p.N = a.N; p.K = a.K;
+  p.a = a.x; p.lda = a.ldx;
+  p.b = a.w; p.ldb = a.ldw;
+  p.c = a.y; p.ldc = a.ldy;
+  p.bias = a.bias; p.res = a.res; p.ldr = a.ldr; p.pre = a.pre; p.ldp = a.ldp;
+  p.act = a.act;
+  return p;
+}
+struct BwdPlan {
+  MmProduct dx, dw;
+  int rows, blocks;
+  long long N4, lddz;
+  size_t dz_bytes, part_bytes, prod_bytes;
+};
+BwdPlan bwd_plan(const LinearBwdArgs& a, void* dz) {
+  BwdPlan b{};
+  const bool own_dz = a.act != ACT_NONE && (a.dx || a.dw);
+  b.N4 = ((long long)a.N + 3) / 4 * 4;
+  b.lddz = ((long long)a.N + 7) / 8 * 8;
+  b.rows = dz_rows(a.M, a.N);
+  b.blocks = ceil_div(a.M, b.rows);
+  b.dz_bytes = own_dz ? round_up((size_t)a.M * b.lddz * elem_bytes(a.kind)) : 0;
+  b.part_bytes = a.db ? round_up((size_t)b.blocks * b.N4 * sizeof(float)) : 0;
+  const void* src = own_dz ? dz : a.dy;
+  const long long ld = own_dz ? b.lddz : a.lddy;
+  // dx[M,K] = dz[M,N] W^T: W^T(n, k) is n-contiguous where W is [K,N]
+  b.dx.kind = a.kind;
+  b.dx.kc_a = 1; b.dx.kc_b = !a.trans_w;
+  b.dx.M = a.M; b.dx.N = a.K; b.dx.K = a.N;
+  b.dx.a = src; b.dx.lda = ld; b.dx.b = a.w; b.dx.ldb = a.ldw;
+  b.dx.c = a.dx; b.dx.ldc = a.lddx;
+  // dw[K,N] = x^T dz, or [N,K] = dz^T x
+  b.dw.kind = a.kind;
+  b.dw.K = a.M;
+  b.dw.M = a.trans_w ? a.N : a.K; b.dw.N = a.trans_w ? a.K : a.N;
+  b.dw.a = a.trans_w ? src : a.x; b.dw.lda = a.trans_w ? ld : a.ldx;
+  b.dw.b = a.trans_w ? a.x : src; b.dw.ldb = a.trans_w ? a.ldx : ld;
+  b.dw.c = a.dw; b.dw.ldc = a.lddw;
+  b.dw.accumulate = a.accumulate;
+  const size_t x = a.dx ? mm_product_workspace(b.dx) : 0, w = a.dw ? mm_product_workspace(b.dw) : 0;
+  b.prod_bytes = x > w ? x : w;
+  return b;
+}
+}  // namespace
+
+size_t linear_workspace(const LinearArgs& a) { return mm_product_workspace(forward_of(a)); }
+void linear(const LinearArgs& a, void* ws, size_t ws_bytes, hipStream_t stream) { mm_product(forward_of(a), ws, ws_bytes, stream); }
+
+size_t linear_bwd_workspace(const LinearBwdArgs& a) {
+  const BwdPlan b = bwd_plan(a, nullptr);
+  return b.dz_bytes + b.part_bytes + b.prod_bytes;
+}
+
+void linear_bwd(const LinearBwdArgs& a, void* ws, size_t ws_bytes, hipStream_t stream) {
+  char* at = reinterpret_cast<char*>(ws);
+  const BwdPlan b = bwd_plan(a, at);
+  check_ws("linear_bwd", b.dz_bytes + b.part_bytes + b.prod_bytes, ws, ws_bytes);
+  float* part = reinterpret_cast<float*>(at + b.dz_bytes);
+  char* prod = at + b.dz_bytes + b.part_bytes;
+  const LinLaunch& f = lin_launch(a.kind);
+  if ((b.dz_bytes || a.db) && a.N > 0) {
+    if (a.M > 0) {
+      LinDzArgs d{};
+      d.dy = a.dy; d.lddy = a.lddy; d.pre = a.pre; d.ldp = a.ldp;
+      d.dz = b.dz_bytes ? at : nullptr; d.lddz = b.lddz;
+      d.part = a.db ? part : nullptr; d.N4 = b.N4;
+      d.M = a.M; d.N = a.N; d.act = a.act; d.rows_per_block = b.rows;
+      const int v4 = 4 * elem_bytes(a.kind);
+      d.vec = !(a.N & 3) && !(a.lddy & 3) && aligned_to(a.dy, v4) && (a.act == ACT_NONE || (!(a.ldp & 3) && aligned_to(a.pre, v4)));
+      f.dz(d, dim3((unsigned)ceil_div(a.N, 256), (unsigned)b.blocks), stream);
+    }
+    if (a.db) {
+      LinColSumArgs c{};
+      c.part = part; c.N4 = b.N4; c.blocks = b.blocks; c.N = a.N; c.accumulate = a.accumulate; c.db = a.db;
+      f.colsum(c, stream);
+    }
+  }
+  if (a.dx) mm_product(b.dx, prod, b.prod_bytes, stream);
+  if (a.dw) mm_product(b.dw, prod, b.prod_bytes, stream);
+}
+
+}  // namespace dtf

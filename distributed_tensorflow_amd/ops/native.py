@@ -1025,6 +1025,178 @@ def gemm(a, b, *, trans_a=False, trans_b=False, bias=None, relu=False, out=None,
     return out
 
 
+# ----------------------------------------------------------------------------- dense layers
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _mat(t: torch.Tensor, what: str, like: torch.Tensor, shape, written: bool = False) -> tuple:
+    """(address, row stride in elements) of a row-strided matrix; shape entries of None are free."""
+    if t.dim() != 2 or any(w is not None and s != w for s, w in zip(t.shape, shape)):
+        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != like.dtype:
+        raise ValueError(f"{what}: expected {like.dtype}, got {t.dtype}")
+    if t.device != like.device:
+        raise ValueError(f"{what}: on {t.device}, expected {like.device}")
+    rows, cols = t.shape
+    ld = t.stride(0) if rows > 1 else cols
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what}: the elements of a row must be contiguous")
+    if written and ld < cols:
+        raise ValueError(f"{what}: rows overlap")
+    if rows >= 2**31 or cols >= 2**31:
+        raise ValueError(f"{what}: a dimension passes 2^31")
+    return t.data_ptr(), ld
+
+
+def _check_device(t: torch.Tensor, what: str) -> None:
+    if t.dtype not in _KINDS:
+        raise ValueError(f"{what}: float32, bfloat16 or float16 tensors, got {t.dtype}")
+    require()
+    if not t.is_cuda:
+        raise ValueError(f"{what}: expected GPU tensors")
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{what}: the tensors are on {t.device}, the current device is {torch.cuda.current_device()}")
+
+
+def _span(t: torch.Tensor) -> tuple:
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _check_apart(what: str, written, read, in_place=()) -> None:
+    """Refuses an output that overlaps an input or another output; `in_place` tensors may be an output itself."""
+    outs = [t for t in written if t is not None]
+    for i, o in enumerate(outs):
+        lo, hi = _span(o)
+        for t in [r for r in read if r is not None] + outs[i + 1:]:
+            a, b = _span(t)
+            if a < hi and lo < b:
+                raise ValueError(f"{what}: an output overlaps another tensor of the call")
+        for t in in_place:
+            if t is None:
+                continue
+            a, b = _span(t)
+            if a < hi and lo < b and not (o is outs[0] and t.data_ptr() == o.data_ptr() and t.stride() == o.stride()):
+                raise ValueError(f"{what}: an output overlaps another tensor of the call")
+
+
+def _workspace(what: str, need: int, workspace: Optional[torch.Tensor], device) -> tuple:
+    """(tensor, address, bytes): the caller's workspace, or one from torch's allocator for the current stream."""
+    if workspace is not None:
+        if workspace.device != device or not workspace.is_contiguous() or workspace.data_ptr() % 16:
+            raise ValueError(f"{what}: the workspace must be contiguous, 16-byte aligned and on the tensors' device")
+        have = workspace.numel() * workspace.element_size()
+        if have < need:
+            raise ValueError(f"{what}: the workspace has {have} bytes, {need} are needed")
+        return workspace, workspace.data_ptr(), have
+    if need == 0:
+        return None, 0, 0
+    if hip().recording():
+        raise ValueError(f"{what}: a recorded call needs a workspace that lives as long as the program ({need} bytes)")
+    ws = torch.empty(need, device=device, dtype=torch.uint8)
+    return ws, ws.data_ptr(), need
+
+
+def linear(x, w, bias=None, *, activation: str = "none", residual=None, trans_w: bool = False, out=None, pre=None, workspace=None):
+    """y = act(x W + bias) + residual in one product with a fused epilogue (csrc/kernels/linear.hip).
+
+    x [M,K]; w [K,N], or [N,K] with trans_w; bias [N]; residual [M,N], added after the activation. All of one
+    type, float32, bfloat16 or float16; sums are fp32 (float32 products run on the exact fp32 matrix pipe) and every
+    output is rounded once. Matrices may be row-strided views. activation: none, relu, gelu (erf), gelu_tanh, silu.
+    pre [M,N] receives x W + bias for linear_bwd. out may be `residual` itself, otherwise outputs overlap nothing.
+    workspace: linear_workspace() bytes; a call recorded into a step program has to bring its own."""
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"linear: unknown activation {activation!r}")
+    px, ldx = _mat(x, "linear: x", x, (None, None))
+    m, k = x.shape
+    pw, ldw = _mat(w, "linear: w", x, (None, k) if trans_w else (k, None))
+    n = w.shape[0] if trans_w else w.shape[1]
+    pb = pr = pp = ldr = ldp = 0
+    if bias is not None:
+        if tuple(bias.shape) != (n,) or bias.dtype != x.dtype or bias.device != x.device or (n > 1 and bias.stride(0) != 1):
+            raise ValueError(f"linear: bias must be a contiguous {x.dtype} vector of {n} on {x.device}")
+        pb = bias.data_ptr()
+    if residual is not None:
+        pr, ldr = _mat(residual, "linear: residual", x, (m, n))
+    if out is None:
+        out = torch.empty((m, n), device=x.device, dtype=x.dtype)
+        if pre is not None:
+            _check_apart("linear", (pre,), (x, w, bias, residual))
+    else:
+        _check_apart("linear", (out, pre), (x, w, bias), (residual,))
+    py, ldy = _mat(out, "linear: out", x, (m, n), written=True)
+    if pre is not None:
+        pp, ldp = _mat(pre, "linear: pre", x, (m, n), written=True)
+    _check_device(x, "linear")
+    args = (_KINDS[x.dtype], m, n, k, int(trans_w), act, px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pp, ldp)
+    ws, addr, have = _workspace("linear", _hip.linear_workspace(*args), workspace, x.device)
+    _hip.linear(*args, addr, have, stream())
+    return out
+
+
+def linear_bwd(dy, x, w, *, pre=None, activation: str = "none", trans_w: bool = False, dx=True, dw=True, db=True,
+               accumulate: bool = False, workspace=None):
+    """Gradients of linear(): dz = dy act'(pre); dx = dz W^T, dw = x^T dz (laid out like w), db = column sums of dz.
+
+    dy [M,N]; pre [M,N] as linear stored it (not needed for activation "none"). The residual's gradient is dy.
+    dx / dw / db: True allocates the output, a tensor receives it, False or None leaves it out. accumulate=True adds
+    to the dw and db that are given (dx is always written). dz is rounded to the tensors' type before the two
+    products (exact for none and relu); db sums the unrounded values. Returns (dx, dw, db), None where left out."""
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"linear_bwd: unknown activation {activation!r}")
+    pdy, lddy = _mat(dy, "linear_bwd: dy", dy, (None, None))
+    m, n = dy.shape
+    px, ldx = _mat(x, "linear_bwd: x", dy, (m, None))
+    k = x.shape[1]
+    wshape = (n, k) if trans_w else (k, n)
+    pw, ldw = _mat(w, "linear_bwd: w", dy, wshape)
+    pp = ldp = 0
+    if act:
+        if pre is None:
+            raise ValueError("linear_bwd: the gradient of an activation needs pre")
+        pp, ldp = _mat(pre, "linear_bwd: pre", dy, (m, n))
+    if accumulate and (dw is True or db is True):
+        raise ValueError("linear_bwd: accumulate=True adds to tensors that are given")
+    given = [t for t in (dx, dw, db) if isinstance(t, torch.Tensor)]
+    if given:
+        _check_apart("linear_bwd", given, (dy, x, w, pre if act else None))
+
+    def output(t, shape):
+        if t is True:
+            return torch.empty(shape, device=dy.device, dtype=dy.dtype)
+        return t if isinstance(t, torch.Tensor) else None
+
+    dx, dw, db = output(dx, (m, k)), output(dw, wshape), output(db, (n,))
+    pdx, lddx = _mat(dx, "linear_bwd: dx", dy, (m, k), written=True) if dx is not None else (0, 0)
+    pdw, lddw = _mat(dw, "linear_bwd: dw", dy, wshape, written=True) if dw is not None else (0, 0)
+    pdb = 0
+    if db is not None:
+        if tuple(db.shape) != (n,) or db.dtype != dy.dtype or db.device != dy.device or (n > 1 and db.stride(0) != 1):
+            raise ValueError(f"linear_bwd: db must be a contiguous {dy.dtype} vector of {n} on {dy.device}")
+        pdb = db.data_ptr()
+    _check_device(dy, "linear_bwd")
+    args = (_KINDS[dy.dtype], m, n, k, int(trans_w), act, int(accumulate), pdy, lddy, pp, ldp, px, ldx, pw, ldw, pdx, lddx, pdw, lddw, pdb)
+    ws, addr, have = _workspace("linear_bwd", _hip.linear_bwd_workspace(*args), workspace, dy.device)
+    _hip.linear_bwd(*args, addr, have, stream())
+    return dx, dw, db
+
+
+def linear_workspace(m: int, n: int, k: int, dtype=torch.float32, trans_w: bool = False) -> int:
+    """Bytes of workspace that linear() may need for x [m,k] and n outputs, whatever the tensors' strides."""
+    return hip().linear_workspace(_KINDS[dtype], m, n, k, int(trans_w), 0, 0, k, 0, k if trans_w else n, 0, 0, 0, 0, n, 0, 0)
+
+
+def linear_bwd_workspace(m: int, n: int, k: int, dtype=torch.float32, trans_w: bool = False, activation: str = "none") -> int:
+    """Bytes of workspace that linear_bwd() may need for dy [m,n] and x [m,k] with all three gradients."""
+    ldw = k if trans_w else n
+    return hip().linear_bwd_workspace(_KINDS[dtype], m, n, k, int(trans_w), ACTIVATIONS[activation], 0, 0, n, 0, n, 0, k, 0, ldw, 1, k, 1, ldw, 1)
+
+
 def col_sum(x2d, out, relu_of=None, masked=None):
     """out[C] += column sums of x2d. relu_of (same shape): sums x2d * 1[relu_of > 0] instead - the
     ReLU backward of x2d - and stores that masked tensor to `masked` when given (x2d itself is fine)."""
