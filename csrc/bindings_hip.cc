@@ -14,6 +14,7 @@
 #include "comm/link_probe.h"
 #include "kernels/conv.h"
 #include "kernels/linear.h"
+#include "kernels/newton_schulz.h"
 #include "kernels/ops.h"
 #include "runtime/program.h"
 
@@ -522,6 +523,47 @@ PYBIND11_MODULE(_hip, m) {
                               long long lddw, uint64_t db, uint64_t ws, size_t ws_bytes, uint64_t stream) {
       linear_bwd(bwd(kind, M, N, K, trans_w, act, accumulate, dy, lddy, pre, ldp, x, ldx, w, ldw, dx, lddx, dw, lddw, db),
                  reinterpret_cast<void*>(ws), ws_bytes, as_stream(stream));
+    });
+  }
+  // Newton-Schulz orthogonalisation: coeffs holds (a, b, c) of every step
+  {
+    auto coeffs = [](const std::vector<float>& v, NsCoeffs* out, int& steps) {
+      if (v.size() % 3 || v.size() / 3 < 1 || v.size() / 3 > (size_t)kNsMaxSteps) throw std::runtime_error("newton_schulz: 1..16 steps of three coefficients");
+      steps = (int)(v.size() / 3);
+      for (int k = 0; k < steps; ++k) out[k] = NsCoeffs{v[3 * k], v[3 * k + 1], v[3 * k + 2]};
+    };
+    m.def("newton_schulz_workspace", [](int kind, int batch, int rows, int cols) {
+      NsArgs a{};
+      a.kind = kind; a.batch = batch; a.rows = rows; a.cols = cols;
+      return ns_workspace(a);
+    });
+    m.def("newton_schulz", [coeffs](int kind, int batch, int rows, int cols, uint64_t g, long long ld, long long g_stride, uint64_t out,
+                                    long long out_ld, long long out_stride, double eps, const std::vector<float>& co, float growth, uint64_t ws,
+                                    size_t ws_bytes, uint64_t stream) {
+      NsArgs a{};
+      a.kind = kind; a.batch = batch; a.rows = rows; a.cols = cols;
+      a.g = reinterpret_cast<const void*>(g); a.ld = ld; a.g_stride = g_stride;
+      a.out = reinterpret_cast<void*>(out); a.out_ld = out_ld; a.out_stride = out_stride;
+      a.eps = eps; a.growth = growth;
+      coeffs(co, a.coeffs, a.steps);
+      newton_schulz(a, reinterpret_cast<void*>(ws), ws_bytes, as_stream(stream));
+    });
+    m.def("ns_shape", [](int rows, int cols) {
+      NsMat x{};
+      ns_shape(x, rows, cols);
+      return py::make_tuple(x.r, x.c, x.rp, x.cp, x.tall, x.parts, x.chunk, x.sx, ns_floats(x));
+    });
+    m.attr("NS_MAT_BYTES") = (int)sizeof(NsMat);
+    m.attr("MUON_TILE") = kMuonTile;
+    m.attr("MUON_VEC_CHUNK") = kMuonVecChunk;
+    m.attr("MUON_VEC_ALIGN") = kMuonVecAlign;
+    m.def("muon_step", [coeffs](const py::dict& d, uint64_t stream) {
+      MuonArgs a{};
+      P(p, float); P(g, const float); P(m, float); P(v, float); P(hyper, const float); P(mats, const NsMat);
+      P(items_flat, const NsItem); P(items_split, const NsItem); P(items_sym, const NsItem); P(items_apply, const NsItem);
+      V(n_flat); V(n_split); V(n_sym); V(n_apply); V(nesterov); V(eps); V(growth);
+      coeffs(d["coeffs"].cast<std::vector<float>>(), a.coeffs, a.steps);
+      muon_step(a, as_ptr<void>(d, "ws"), as_stream(stream));
     });
   }
   m.def("col_sum", [](const py::dict& d, uint64_t stream) {

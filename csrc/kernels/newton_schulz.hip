@@ -1,0 +1,414 @@
+// Newton-Schulz orthogonalisation on the fp16 matrix pipe with operands kept as pairs of fp16 numbers.
+//
+// Precision: five steps amplify a rounding error in a direction of a small singular value 485-fold. Single bf16 or fp16
+// operands leave errors of 3 - 30 % / 0.4 - 4 % in the result; h + l with 22 bits and the three products hh + hl + lh (mm_tile.h)
+// measures within 10 % of what fp32 products leave (1e-6 - 1e-5 relative, 64x10 to 1024x2048). Everything is scaled by powers
+// of two that keep h in fp16's normal range: X by sx ~ sqrt(r c), so that typical elements of X_0 are about 1, A and P by 2^12.
+// A matrix whose norm is far below eps starts with tiny X_0; its part below one is carried apart in tau (a power of two per
+// matrix, grown by `growth` per step up to 1), so that the fp16 numbers never see it: X = tau Xs,
+//   Xs <- (tau / tau') (a I + b tau^2 As + c tau^4 As^2) Xs.
+//
+// A step is three products: A = X X^T and P = a I + b A + c A^2 are symmetric, so only the tiles on and below the diagonal are
+// computed and each is stored twice; X' = P X. The last one writes the output (or updates the parameter) directly.
+#include "newton_schulz.h"
+#include "mm_tile.h"
+
+namespace dtf {
+namespace {
+
+constexpr float kScaleA = 4096.f, kScaleP = 4096.f;   // |A| <= 3.8^2 and |P| <= 14 stay below fp16's 65504
+
+struct NsDev {
+  NsMat one;                   // table == nullptr: `batch` matrices of this shape
+  const NsMat* table;
+  const NsItem* items;
+  int total, per_mat;          // items in all, and per matrix
+  long long g_stride, out_stride, ws_stride;
+  float* ws;
+  const void* g;               // fp32 / bf16 / fp16
+  void* out;
+  int kind;
+  float* m;                    // optimizer: momentum, updated in place; g is then the raw gradient
+  float* v;                    // optimizer: second moments of the vectors
+  const float* hyper;
+  int nesterov;
+  double eps;
+  int step, last;
+  float growth;
+  NsCoeffs co;
+};
+
+__device__ __forceinline__ void ns_find(const NsDev& a, int t, NsMat& m, int& tile) {
+  if (a.table) {
+    const NsItem it = a.items[t];
+    m = a.table[it.mat];
+    tile = it.tile;
+  } else {
+    const int b = t / a.per_mat;
+    tile = t - b * a.per_mat;
+    m = a.one;
+    m.src += b * a.g_stride;
+    m.out += b * a.out_stride;
+    m.ws += b * a.ws_stride;
+  }
+}
+__device__ __forceinline__ float ns_read(const void* g, int kind, long long i) {
+  if (kind == MM_F32) return reinterpret_cast<const float*>(g)[i];
+  if (kind == MM_BF16) return (float)reinterpret_cast<const __bf16*>(g)[i];
+  return (float)reinterpret_cast<const _Float16*>(g)[i];
+}
+
+// Sum over a block of 256 in a fixed order; every thread gets it.
+__device__ __forceinline__ double block_sum(double v, double* scratch) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
+}
+
+// Squares of one chunk of G, in 64 bits (squares of gradients leave fp32's range).
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsDev a) {
+  __shared__ double scratch[4];
+  NsMat m;
+  int chunk;
+  ns_find(a, blockIdx.x, m, chunk);
+  const long long n = (long long)m.rows * m.cols;
+  const long long lo = (long long)chunk * m.chunk, hi = min(n, lo + m.chunk);
+  double s = 0.0;
+  for (long long i = lo + threadIdx.x; i < hi; i += 256) {
+    const long long row = i / m.cols;
+    const float x = ns_read(a.g, a.kind, m.src + row * m.ld + (i - row * m.cols));
+    s += (double)x * x;
+  }
+  s = block_sum(s, scratch);
+  if (threadIdx.x == 0) reinterpret_cast<double*>(a.ws + m.ws)[chunk] = s;
+}
+
+// The optimizer's elementwise pass: momentum and the norm of the update for a chunk of a matrix, Adam for a piece of a vector.
+__global__ __launch_bounds__(256) void muon_flat_kernel(NsDev a) {
+  __shared__ double scratch[4];
+  const NsItem it = a.items[blockIdx.x];
+  const float mu = a.hyper[1], gs = a.hyper[2];
+  const float* g = reinterpret_cast<const float*>(a.g);
+  if (it.mat < 0) {
+    const int n = -1 - it.mat;
+    const float lr_t = a.hyper[4], c1 = a.hyper[5], c2 = a.hyper[6], eps = a.hyper[7];
+    float* p = reinterpret_cast<float*>(a.out);
+    for (int k = threadIdx.x; k < n; k += 256) {
+      const long long i = (long long)it.tile * kMuonVecAlign + k;
+      const float x = g[i] * gs;
+      const float m = (1.f - c1) * a.m[i] + c1 * x;
+      const float v = (1.f - c2) * a.v[i] + c2 * x * x;
+      a.m[i] = m;
+      a.v[i] = v;
+      p[i] -= lr_t * m / (sqrtf(v) + eps);
+    }
+    return;
+  }
+  const NsMat m = a.table[it.mat];
+  const long long n = (long long)m.rows * m.cols;
+  const long long lo = (long long)it.tile * m.chunk, hi = min(n, lo + m.chunk);
+  double s = 0.0;
+  for (long long i = lo + threadIdx.x; i < hi; i += 256) {
+    const float x = g[m.src + i] * gs;
+    const float mom = mu * a.m[m.src + i] + x;
+    a.m[m.src + i] = mom;
+    const float u = a.nesterov ? x + mu * mom : mom;
+    s += (double)u * u;
+  }
+  s = block_sum(s, scratch);
+  if (threadIdx.x == 0) reinterpret_cast<double*>(a.ws + m.ws)[it.tile] = s;
+}
+
+__device__ __forceinline__ float tau_at(float tau0, float growth, int step) {
+  float t = tau0;
+  for (int k = 0; k < step; ++k) t = fminf(1.f, t * growth);
+  return t;
+}
+
+// h and l of four values at (row, col..col+3), col a multiple of 4
+__device__ __forceinline__ char* pair_at(float* base, int pitch, int row, int col) {
+  return reinterpret_cast<char*>(base + (long long)row * pitch + (col & ~31)) + (col & 31) * 2;
+}
+__device__ __forceinline__ void pair_split(const floatx4& v, halfx4& h, halfx4& l) {
+  h = __builtin_convertvector(v, halfx4);
+  const floatx4 rest = v - __builtin_convertvector(h, floatx4);   // exact
+  l = __builtin_convertvector(rest, halfx4);
+}
+__device__ __forceinline__ void pair_store4(float* base, int pitch, int row, int col, const floatx4& v) {
+  halfx4 h, l;
+  pair_split(v, h, l);
+  char* p = pair_at(base, pitch, row, col);
+  *reinterpret_cast<halfx4*>(p) = h;
+  *reinterpret_cast<halfx4*>(p + 64) = l;
+}
+__device__ __forceinline__ floatx4 pair_load4(const float* base, int pitch, int row, int col) {
+  const char* p = pair_at(const_cast<float*>(base), pitch, row, col);
+  return __builtin_convertvector(*reinterpret_cast<const halfx4*>(p), floatx4) + __builtin_convertvector(*reinterpret_cast<const halfx4*>(p + 64), floatx4);
+}
+
+// G / (|G| + eps) / tau as pairs, one 32 x 32 block of X per workgroup (transposed on the way where G is tall).
+__global__ __launch_bounds__(256) void ns_split_kernel(NsDev a) {
+  __shared__ double scratch[4];
+  __shared__ float block[32][33];
+  NsMat m;
+  int tile;
+  ns_find(a, blockIdx.x, m, tile);
+  float* base = a.ws + m.ws;
+  const double* parts = reinterpret_cast<const double*>(base);
+  const double ss = block_sum((int)threadIdx.x < m.parts ? parts[threadIdx.x] : 0.0, scratch);
+  const double norm = sqrt(ss), t = norm / (norm + a.eps);
+  // tau: the power of two at or above t, 1 unless the norm is below eps (or is not a number)
+  float tau = 1.f;
+  if (t < 0.5) tau = t > 1e-37 ? ldexpf(1.f, ilogb(t) + 1) : 1.1754944e-38f;
+  const double inv = (double)m.sx / ((norm + a.eps) * (double)tau);
+  const int bc = m.cp / 32, bi = tile / bc, bj = tile - bi * bc;   // block of X
+  if (tile == 0 && threadIdx.x == 0) base[2 * kNsNormParts] = tau;
+  const int r0 = (m.tall ? bj : bi) * 32, c0 = (m.tall ? bi : bj) * 32;   // block of G
+  const float mu = a.m ? a.hyper[1] : 0.f, gs = a.m ? a.hyper[2] : 1.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int y = (threadIdx.x >> 5) + 8 * k, x = threadIdx.x & 31;
+    float v = 0.f;
+    if (r0 + y < m.rows && c0 + x < m.cols) {
+      const long long i = m.src + (long long)(r0 + y) * m.ld + c0 + x;
+      v = ns_read(a.g, a.kind, i);
+      if (a.m) {
+        const float mom = a.m[i];
+        v = a.nesterov ? v * gs + mu * mom : mom;
+      }
+      v = (float)((double)v * inv);
+    }
+    if (m.tall) block[x][y] = v;
+    else block[y][x] = v;
+  }
+  __syncthreads();
+  const int y = threadIdx.x >> 3, x = (threadIdx.x & 7) * 4;
+  pair_store4(a.ws + ns_x(m), m.cp, bi * 32 + y, bj * 32 + x, floatx4{block[y][x], block[y][x + 1], block[y][x + 2], block[y][x + 3]});
+}
+
+enum NsOp { NS_GRAM, NS_POLY, NS_APPLY };
+
+template <int T, bool KCB, bool SWAP>
+using NsLoop = MmRegs<MM_PAIR, true, KCB, T, T, 2, 2, SWAP>;
+
+// One T x T tile of one of the three products.
+template <NsOp OP, int T>
+__global__ __launch_bounds__(256) void ns_product_kernel(NsDev a) {
+  extern __shared__ __attribute__((aligned(16))) char ns_smem[];
+  const int t = mm_item(blockIdx.x, a.total);
+  if (t >= a.total) return;
+  NsMat m;
+  int tile;
+  ns_find(a, t, m, tile);
+  int tx, ty;
+  if (OP == NS_APPLY) {
+    mm_tile_of(tile, (m.cp + T - 1) / T, (m.rp + T - 1) / T, tx, ty);
+  } else {   // lower triangle, row by row
+    ty = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+    while ((ty + 1) * (ty + 2) / 2 <= tile) ++ty;
+    while (ty * (ty + 1) / 2 > tile) --ty;
+    tx = tile - ty * (ty + 1) / 2;
+  }
+  const int m0 = ty * T, n0 = tx * T;
+  float *xa = a.ws + ns_x(m), *xb = xa + ns_x_floats(m);
+  if (a.step & 1) { float* s = xa; xa = xb; xb = s; }
+  float *A = a.ws + ns_a(m), *P = a.ws + ns_p(m);
+
+  constexpr int MI = T / 32, NJ = T / 32;
+  floatx4 acc[MI][NJ];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, l15 = lane & 15;
+  const int wm = (wave >> 1) * (T / 2), wn = (wave & 1) * (T / 2);
+
+  if (OP != NS_APPLY) {
+    const float* src = OP == NS_GRAM ? xa : A;
+    const int pitch = OP == NS_GRAM ? m.cp : m.rp;
+    const char* s = reinterpret_cast<const char*>(src);
+    NsLoop<T, true, true>::run(MmOperands{s, s, pitch, pitch, m.rp, m.rp}, m0, n0, 0, pitch, ns_smem, acc);
+    float* dst = OP == NS_GRAM ? A : P;
+    float ca = 0.f, cb = 0.f, cc;   // value = ca I + cb A + cc acc
+    if (OP == NS_GRAM) {
+      cc = kScaleA / (m.sx * m.sx);
+    } else {
+      const float tau = tau_at(a.ws[m.ws + 2 * kNsNormParts], a.growth, a.step), next = fminf(1.f, tau * a.growth);
+      const float s1 = kScaleP * (tau / next), t2 = tau * tau;
+      ca = s1 * a.co.a;
+      cb = s1 * a.co.b * t2 * (1.f / kScaleA);
+      cc = s1 * a.co.c * t2 * t2 * (1.f / (kScaleA * kScaleA));
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int mm = m0 + wm + i * 16 + l15;
+      if (mm >= m.rp) continue;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int nn = n0 + wn + j * 16 + 4 * q;
+        if (nn >= m.rp) continue;
+        floatx4 v = acc[i][j] * cc;
+        if (OP == NS_POLY) {
+          v += pair_load4(A, m.rp, mm, nn) * cb;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (mm == nn + e && mm < m.r) v[e] += ca;
+        }
+        pair_store4(dst, m.rp, mm, nn, v);
+        if (m0 != n0) {   // the mirrored tile
+          halfx4 h, l;
+          pair_split(v, h, l);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            _Float16* p = reinterpret_cast<_Float16*>(dst + (long long)(nn + e) * m.rp + (mm & ~31)) + (mm & 31);
+            p[0] = h[e];
+            p[32] = l[e];
+          }
+        }
+      }
+    }
+    return;
+  }
+
+  const MmOperands o{reinterpret_cast<const char*>(P), reinterpret_cast<const char*>(xa), m.rp, m.cp, m.rp, m.cp};
+  if (!a.last || !m.tall) NsLoop<T, false, true>::run(o, m0, n0, 0, m.rp, ns_smem, acc);
+  else NsLoop<T, false, false>::run(o, m0, n0, 0, m.rp, ns_smem, acc);
+  if (!a.last) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int mm = m0 + wm + i * 16 + l15;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int nn = n0 + wn + j * 16 + 4 * q;
+        if (mm < m.rp && nn < m.cp) pair_store4(xb, m.cp, mm, nn, acc[i][j] * (1.f / kScaleP));
+      }
+    }
+    return;
+  }
+  // The output, in G's orientation: a lane holds four consecutive elements of a row of it.
+  const float tau = tau_at(a.ws[m.ws + 2 * kNsNormParts], a.growth, a.step + 1);
+  const float f = tau / (kScaleP * m.sx);
+  const float lr = a.m ? a.hyper[0] * m.scale : 0.f, decay = a.m ? a.hyper[3] : 0.f;
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int row = m.tall ? n0 + wn + j * 16 + l15 : m0 + wm + i * 16 + l15;
+      const int col = (m.tall ? m0 + wm + i * 16 : n0 + wn + j * 16) + 4 * q;
+      if (row >= m.rows) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (col + e >= m.cols) continue;
+        const long long at = m.out + (long long)row * m.out_ld + col + e;
+        const float v = acc[i][j][e] * f;
+        if (a.m) {
+          float* p = reinterpret_cast<float*>(a.out) + at;
+          *p = decay * *p - lr * v;
+        } else if (a.kind == MM_F32) {
+          reinterpret_cast<float*>(a.out)[at] = v;
+        } else if (a.kind == MM_BF16) {
+          reinterpret_cast<__bf16*>(a.out)[at] = (__bf16)v;
+        } else {
+          reinterpret_cast<_Float16*>(a.out)[at] = (_Float16)v;
+        }
+      }
+    }
+}
+
+template <NsOp OP>
+void product(const char* name, NsDev d, int tile, hipStream_t stream) {
+  const dim3 grid((unsigned)((d.total + 7) / 8 * 8));
+  if (tile == 128) launch(name, ns_product_kernel<OP, 128>, grid, dim3(256), NsLoop<128, true, true>::LDS, stream, d);
+  else launch(name, ns_product_kernel<OP, 64>, grid, dim3(256), NsLoop<64, true, true>::LDS, stream, d);
+}
+
+int sym_tiles(const NsMat& m, int T) { const int t = ceil_div(m.rp, T); return t * (t + 1) / 2; }
+int apply_tiles(const NsMat& m, int T) { return ceil_div(m.rp, T) * ceil_div(m.cp, T); }
+
+}  // namespace
+
+void ns_shape(NsMat& m, int rows, int cols) {
+  m.rows = rows; m.cols = cols;
+  m.tall = rows > cols;
+  m.r = rows < cols ? rows : cols;
+  m.c = rows < cols ? cols : rows;
+  m.rp = ceil_div(m.r, 32) * 32;
+  m.cp = ceil_div(m.c, 32) * 32;
+  const long long n = (long long)rows * cols;
+  const long long chunk = (n + kNsNormParts - 1) / kNsNormParts;
+  m.chunk = (int)(chunk < 2048 ? 2048 : chunk);
+  m.parts = (int)((n + m.chunk - 1) / m.chunk);
+  float s = 1.f;
+  while (s * s < (float)n && s < 8192.f) s *= 2.f;   // the iterates stay below 3.8: 3.8 * 8192 is inside fp16's range
+  m.sx = s;
+}
+
+size_t ns_workspace(const NsArgs& a) {
+  NsMat m{};
+  ns_shape(m, a.rows, a.cols);
+  return (size_t)ns_floats(m) * sizeof(float) * a.batch;
+}
+
+void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t stream) {
+  if (a.batch <= 0 || a.rows <= 0 || a.cols <= 0) return;
+  if (a.steps < 1 || a.steps > kNsMaxSteps) throw std::runtime_error("newton_schulz: 1..16 steps");
+  if (ns_workspace(a) > ws_bytes || !ws || (reinterpret_cast<uintptr_t>(ws) & 15)) throw std::runtime_error("newton_schulz: workspace too small or unaligned");
+  NsDev d{};
+  ns_shape(d.one, a.rows, a.cols);
+  d.one.ld = a.ld; d.one.out_ld = a.out_ld;
+  d.g = a.g; d.out = a.out; d.kind = a.kind;
+  d.g_stride = a.g_stride; d.out_stride = a.out_stride; d.ws_stride = ns_floats(d.one);
+  d.ws = reinterpret_cast<float*>(ws);
+  d.eps = a.eps; d.growth = a.growth;
+  const NsMat& m = d.one;
+  auto with = [&](int per) {
+    if ((long long)per * a.batch > 0x3fffffff) throw std::runtime_error("newton_schulz: too many tiles");
+    NsDev x = d;
+    x.per_mat = per;
+    x.total = per * a.batch;
+    return x;
+  };
+  const NsDev n = with(m.parts);
+  launch("ns_norm", ns_norm_kernel, dim3(n.total), dim3(256), 0, stream, n);
+  const NsDev s = with((m.rp / 32) * (m.cp / 32));
+  launch("ns_split", ns_split_kernel, dim3(s.total), dim3(256), 0, stream, s);
+  const int tile = (long long)apply_tiles(m, 128) * a.batch >= 128 ? 128 : 64;
+  for (int k = 0; k < a.steps; ++k) {
+    d.step = k;
+    d.last = k == a.steps - 1;
+    d.co = a.coeffs[k];
+    product<NS_GRAM>("ns_gram", with(sym_tiles(m, tile)), tile, stream);
+    product<NS_POLY>("ns_poly", with(sym_tiles(m, tile)), tile, stream);
+    product<NS_APPLY>("ns_apply", with(apply_tiles(m, tile)), tile, stream);
+  }
+}
+
+void muon_step(const MuonArgs& a, void* ws, hipStream_t stream) {
+  if (a.steps < 1 || a.steps > kNsMaxSteps) throw std::runtime_error("muon_step: 1..16 steps");
+  NsDev d{};
+  d.table = a.mats;
+  d.ws = reinterpret_cast<float*>(ws);
+  d.g = a.g; d.out = a.p; d.m = a.m; d.v = a.v; d.hyper = a.hyper; d.kind = MM_F32;
+  d.nesterov = a.nesterov; d.eps = a.eps; d.growth = a.growth;
+  auto with = [&](const NsItem* items, int total) {
+    NsDev x = d;
+    x.items = items;
+    x.total = total;
+    return x;
+  };
+  if (a.n_flat > 0) launch("muon_flat", muon_flat_kernel, dim3(a.n_flat), dim3(256), 0, stream, with(a.items_flat, a.n_flat));
+  if (a.n_split <= 0) return;
+  launch("muon_split", ns_split_kernel, dim3(a.n_split), dim3(256), 0, stream, with(a.items_split, a.n_split));
+  for (int k = 0; k < a.steps; ++k) {
+    d.step = k;
+    d.last = k == a.steps - 1;
+    d.co = a.coeffs[k];
+    product<NS_GRAM>("muon_gram", with(a.items_sym, a.n_sym), kMuonTile, stream);
+    product<NS_POLY>("muon_poly", with(a.items_sym, a.n_sym), kMuonTile, stream);
+    product<NS_APPLY>("muon_apply", with(a.items_apply, a.n_apply), kMuonTile, stream);
+  }
+}
+
+}  // namespace dtf

@@ -8,13 +8,15 @@ instead of silently falling back to PyTorch ops.
 """
 from __future__ import annotations
 
+import functools
+import math
 from dataclasses import dataclass
 from typing import Dict, Optional
 
 import numpy as np
 import torch
 
-from .reference import BN_EPSILON, same_pad
+from .reference import BN_EPSILON, NS_COEFFS, same_pad
 
 try:  # the .so is built in-tree by build_native.py
     from .. import _hip  # type: ignore
@@ -1184,6 +1186,136 @@ def linear_bwd(dy, x, w, *, pre=None, activation: str = "none", trans_w: bool = 
     ws, addr, have = _workspace("linear_bwd", _hip.linear_bwd_workspace(*args), workspace, dy.device)
     _hip.linear_bwd(*args, addr, have, stream())
     return dx, dw, db
+
+
+NS_MAX_STEPS = 16
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_steps(coeffs: tuple, steps: int) -> tuple:
+    """(flat coefficients of every step, growth). Singular values start at or below 1 and go through
+    s (a + b s^2 + c s^4) per step; the kernels hold iterates up to 3.8 and factors up to 14."""
+    if not 1 <= steps <= NS_MAX_STEPS:
+        raise ValueError(f"newton_schulz: 1 to {NS_MAX_STEPS} steps, got {steps}")
+    per_step = coeffs if isinstance(coeffs[0], tuple) else (coeffs,) * steps
+    if len(per_step) != steps or any(len(c) != 3 or not all(math.isfinite(v) for v in c) for c in per_step):
+        raise ValueError("newton_schulz: coeffs is (a, b, c), or one such triple for every step")
+    top, factor, flat = 1.001, 1.0, []
+    for a, b, c in per_step:
+        # extremes of s (a + b s^2 + c s^4) and of a + b s^2 + c s^4 over [0, top]: at the ends and where the derivative is zero
+        squares = [top * top]
+        if c:
+            d = 9 * b * b - 20 * a * c
+            if d >= 0:
+                squares += [(-3 * b + r * math.sqrt(d)) / (10 * c) for r in (1, -1)]
+            squares.append(-b / (2 * c))
+        elif b:
+            squares.append(-a / (3 * b))
+        squares = [q for q in squares if 0 <= q <= top * top] + [0.0]
+        factor = max([factor] + [abs(a + b * q + c * q * q) for q in squares])
+        top = 1.001 * max(math.sqrt(q) * abs(a + b * q + c * q * q) for q in squares)
+        if top > 3.8 or factor > 14:
+            raise ValueError(f"newton_schulz: with coefficients {per_step} the iterates grow to {top:.3g} (at most 3.8) or by {factor:.3g} a step (at most 14)")
+        flat += [a, b, c]
+    return flat, 2.0 ** math.ceil(math.log2(factor))
+
+
+def _ns_key(coeffs) -> tuple:
+    return tuple(tuple(float(v) for v in c) for c in coeffs) if isinstance(coeffs[0], (tuple, list)) else tuple(float(v) for v in coeffs)
+
+
+def newton_schulz(g, *, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out=None, workspace=None):
+    """Orthogonalises the matrix g [m,n], or every matrix of g [batch,m,n], by Newton-Schulz steps
+    (csrc/kernels/newton_schulz.hip): X = g / (|g| + eps), then X <- a X + (b A + c A^2) X with A = X X^T.
+
+    float32, bfloat16 or float16 in and out; the products run on fp16 pairs (22 bits) with fp32 sums whatever the
+    type, since five steps amplify an early rounding error up to 485-fold. Rows may be strided. coeffs: (a, b, c), or
+    a triple for every step; sequences whose iterates would leave the pairs' range are refused. out may be g itself.
+    workspace: newton_schulz_workspace() bytes; a call recorded into a step program has to bring its own."""
+    if g.dim() not in (2, 3):
+        raise ValueError("newton_schulz: a matrix or a batch of matrices")
+    if not eps > 0:
+        raise ValueError("newton_schulz: eps must be positive")
+    flat, growth = _ns_steps(_ns_key(coeffs), steps)
+    rows, cols = g.shape[-2:]
+
+    def place(t, what, written):
+        _mat(t if t.dim() == 2 else t[0] if t.shape[0] else t.new_empty(rows, cols), what, g, (rows, cols), written)
+        ld, gap = (t.stride(-2) if rows > 1 else cols), (t.stride(0) if t.dim() == 3 and t.shape[0] > 1 else 0)
+        if written and t.dim() == 3 and t.shape[0] > 1 and not (gap >= ld * (rows - 1) + cols or (gap >= cols and ld >= gap * (t.shape[0] - 1) + cols)):
+            raise ValueError(f"{what}: the matrices overlap")
+        return t.data_ptr(), ld, gap
+
+    pg = place(g, "newton_schulz: g", False)
+    if out is None:
+        out = torch.empty(g.shape, device=g.device, dtype=g.dtype)
+    elif out.shape != g.shape:
+        raise ValueError(f"newton_schulz: out has shape {tuple(out.shape)}, expected {tuple(g.shape)}")
+    po = place(out, "newton_schulz: out", True)
+    _check_device(g, "newton_schulz")
+    if g.numel() == 0:
+        return out
+    batch = g.shape[0] if g.dim() == 3 else 1
+    kind = _KINDS[g.dtype]
+    ws, addr, have = _workspace("newton_schulz", _hip.newton_schulz_workspace(kind, batch, rows, cols), workspace, g.device)
+    _hip.newton_schulz(kind, batch, rows, cols, *pg, *po, eps, flat, growth, addr, have, stream())
+    return out
+
+
+def newton_schulz_workspace(m: int, n: int, batch: int = 1) -> int:
+    """Bytes of workspace that newton_schulz() needs for [batch, m, n]."""
+    return hip().newton_schulz_workspace(0, batch, m, n)
+
+
+class MuonTables:
+    """What one optimizer's muon_step launches work from: the matrices of a flat parameter buffer, the work items of every
+    launch and the workspace, on the device. `matrices`: (offset, rows, cols); `vectors`: (offset, elements)."""
+
+    MAT = np.dtype([("src", "<i8"), ("out", "<i8"), ("ld", "<i8"), ("out_ld", "<i8"), ("ws", "<i8"), ("rows", "<i4"), ("cols", "<i4"), ("r", "<i4"),
+                    ("c", "<i4"), ("rp", "<i4"), ("cp", "<i4"), ("tall", "<i4"), ("parts", "<i4"), ("chunk", "<i4"), ("sx", "<f4"), ("scale", "<f4"),
+                    ("pad", "<i4")])
+
+    def __init__(self, matrices, vectors, device):
+        require()
+        h = hip()
+        assert self.MAT.itemsize == h.NS_MAT_BYTES
+        mats = np.zeros(len(matrices), dtype=self.MAT)
+        flat, split, sym, apply, floats, tile = [], [], [], [], 0, h.MUON_TILE
+        for i, (off, rows, cols) in enumerate(matrices):
+            r, c, rp, cp, tall, parts, chunk, sx, need = h.ns_shape(rows, cols)
+            mats[i] = (off, off, cols, cols, floats, rows, cols, r, c, rp, cp, tall, parts, chunk, sx, math.sqrt(max(1.0, cols / rows)), 0)
+            floats += (need + 63) // 64 * 64
+            tr, tc = -(-rp // tile), -(-cp // tile)
+            flat += [(i, k) for k in range(parts)]
+            split += [(i, k) for k in range((rp // 32) * (cp // 32))]
+            sym += [(i, k) for k in range(tr * (tr + 1) // 2)]
+            apply += [(i, k) for k in range(tr * tc)]
+        for off, n in vectors:
+            if off % h.MUON_VEC_ALIGN:
+                raise ValueError("MuonTables: vectors start on multiples of 64 elements")
+            for k in range(0, n, h.MUON_VEC_CHUNK):
+                flat.append((-1 - min(h.MUON_VEC_CHUNK, n - k), (off + k) // h.MUON_VEC_ALIGN))
+        self.workspace = torch.empty(max(1, floats), device=device, dtype=torch.float32)
+        self._mats = torch.from_numpy(mats.view(np.uint8).copy()).to(device)
+        self._items = [torch.tensor(x, dtype=torch.int32).reshape(-1, 2).to(device) for x in (flat, split, sym, apply)]
+
+    def launch_args(self) -> dict:
+        d = dict(mats=self._mats.data_ptr(), ws=self.workspace.data_ptr())
+        for name, t in zip(("flat", "split", "sym", "apply"), self._items):
+            d["items_" + name], d["n_" + name] = t.data_ptr(), t.shape[0]
+        return d
+
+
+def muon_step(p, g, m, v, hyper, tables: MuonTables, *, nesterov: bool, steps: int, coeffs=NS_COEFFS, eps: float = 1e-7):
+    """One orthogonalised-momentum step over a flat buffer (csrc/kernels/newton_schulz.hip). hyper: lr, momentum,
+    grad_scale, 1 - lr * weight_decay, then the vectors' Adam step size, 1 - beta1, 1 - beta2 and epsilon."""
+    require()
+    n = p.numel()
+    if g.numel() != n or m.numel() != n or v.numel() != n or hyper.numel() < HYPER_SLOTS:
+        raise ValueError("muon_step: size mismatch")
+    flat, growth = _ns_steps(_ns_key(coeffs), steps)
+    hip().muon_step(dict(p=_chk(p, "p"), g=_chk(g, "g"), m=_chk(m, "m"), v=_chk(v, "v"), hyper=_chk(hyper, "hyper"), nesterov=int(nesterov),
+                         coeffs=flat, growth=growth, eps=float(eps), **tables.launch_args()), stream())
 
 
 def linear_workspace(m: int, n: int, k: int, dtype=torch.float32, trans_w: bool = False) -> int:

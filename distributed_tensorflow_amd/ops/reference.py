@@ -98,6 +98,33 @@ def momentum_update(p, g, m, lr: float, momentum: float, weight_decay: float = 0
     p.sub_(lr * m)
 
 
+# (a, b, c) of the quintic step commonly used to orthogonalise an optimizer's update
+NS_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def newton_schulz(g: torch.Tensor, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7) -> torch.Tensor:
+    """X_0 = G / (|G| + eps); X <- a X + (b A + c A^2) X with A = X X^T, on the orientation with the fewer rows.
+    coeffs: one triple, or one per step."""
+    per_step = [coeffs] * steps if not isinstance(coeffs[0], (tuple, list)) else list(coeffs)
+    x = g.double() if g.dtype == torch.float64 else g.float()
+    tall = x.shape[0] > x.shape[1]
+    x = x.t() if tall else x
+    x = x / (x.double().norm() + eps).to(x.dtype)
+    for a, b, c in per_step:
+        s = x @ x.t()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return (x.t() if tall else x).to(g.dtype)
+
+
+def muon_update(p, g, m, lr: float, momentum: float, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
+                coeffs=NS_COEFFS, eps: float = 1e-7):
+    """Momentum and an orthogonalised update of one matrix [in, out]; the step is scaled by sqrt(max(1, out / in))."""
+    m.mul_(momentum).add_(g)
+    u = g + momentum * m if nesterov else m
+    o = newton_schulz(u, steps, coeffs, eps)
+    p.mul_(1.0 - lr * weight_decay).sub_(lr * math.sqrt(max(1.0, p.shape[1] / p.shape[0])) * o)
+
+
 def adam_lr_t(lr: float, step: int, beta1: float = 0.9, beta2: float = 0.999) -> float:
     """Step size of update number `step` (1-based)."""
     return lr * math.sqrt(1.0 - beta2 ** step) / (1.0 - beta1 ** step)

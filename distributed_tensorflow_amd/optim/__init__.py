@@ -1,6 +1,6 @@
-"""Optimizers: fused flat-arena Adam / momentum SGD, and the reference's synchronisation wrappers
+"""Optimizers: fused flat-arena Adam / momentum SGD / orthogonalised momentum, and the reference's synchronisation wrappers
 by their original class names."""
-from .flat import FlatAdam, FlatMomentumSGD  # noqa: F401
+from .flat import FlatAdam, FlatMomentumSGD, FlatMuon  # noqa: F401
 from .sync_replicas import (  # noqa: F401
     BackupOptimizer,
     ChiefQueueRunner,

@@ -3,16 +3,18 @@
 `FlatAdam` is tf.train.AdamOptimizer as the reference configures it (beta1 0.9, beta2 0.999,
 epsilon 1e-8, bias correction folded into the step size; reference:
 DistributedLeNet/src/distributed_train.py:164), `FlatMomentumSGD` is momentum SGD with L2 weight
-decay (the `weight_decay` hyper-parameter of DistributedResNet/src/hyper_parameters.py:29).
+decay (the `weight_decay` hyper-parameter of DistributedResNet/src/hyper_parameters.py:29). `FlatMuon`
+orthogonalises the momentum of every weight matrix by Newton-Schulz products and uses Adam for the vectors.
 
-One `step()` is ONE kernel launch over the whole arena on a GPU (csrc/kernels/optim.hip); the
+One `step()` of the first two is ONE kernel launch over the whole arena on a GPU (csrc/kernels/optim.hip); the
 averaging of an aggregated gradient (`grad_scale` = 1 / contributors) happens inside that launch,
 so a summed gradient never needs a separate scaling pass. On a CPU arena the same arithmetic runs
 in PyTorch (ops/reference.py), which is also what the kernels are tested against.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+import math
+from typing import Iterable, List, Optional, Tuple
 
 import torch
 
@@ -93,3 +95,60 @@ class FlatMomentumSGD(_FlatOptimizer):
                 g = a.grads[lo:hi] * grad_scale if grad_scale != 1.0 else a.grads[lo:hi]
                 ref.momentum_update(a.params[lo:hi], g, a.slots["m"][lo:hi], lr, self.momentum, self.weight_decay)
         self.steps += 1
+
+
+class FlatMuon(_FlatOptimizer):
+    """Momentum whose update is orthogonalised, matrix by matrix (ops/reference.py::muon_update): a parameter of two or
+    more dimensions is the matrix [product of the leading dimensions, last dimension], so an HWIO filter is
+    [kh kw in, out]; its step is lr * sqrt(max(1, out / in)) times an update whose singular values are near one, after a
+    decoupled weight decay. Everything else (biases, normalisation parameters, and matrices not named in `matrices`)
+    is updated by Adam with `vector_lr`. Slot "m" holds the momentum of either kind, "v" the vectors' second moments.
+
+    On a GPU a step is 2 + 3 * ns_steps launches whatever the number of parameters: every launch works on all
+    matrices at once from tables built here."""
+
+    slots = ("m", "v")
+
+    def __init__(self, arena: ParamArena, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, ns_steps: int = 5,
+                 ns_coeffs=ref.NS_COEFFS, ns_eps: float = 1e-7, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
+                 matrices: Optional[Iterable[str]] = None):
+        super().__init__(arena)
+        self.momentum, self.nesterov, self.weight_decay = momentum, nesterov, weight_decay
+        self.ns_steps, self.ns_coeffs, self.ns_eps = ns_steps, ns_coeffs, ns_eps
+        self.beta1, self.beta2, self.eps = beta1, beta2, eps
+        named = None if matrices is None else set(matrices)
+        if named is not None and named - set(arena.names()):
+            raise ValueError(f"no parameter is named {sorted(named - set(arena.names()))}")
+        if named is not None and any(len(arena.spec(n).shape) < 2 for n in named):
+            raise ValueError("a matrix has at least two dimensions")
+        self._matrices: List[Tuple[int, int, int]] = []
+        self._vectors: List[Tuple[int, int]] = []
+        for s in arena.specs:
+            off = arena.offsets[s.name]
+            if s.numel == 0:
+                continue
+            if len(s.shape) >= 2 and (named is None or s.name in named):
+                self._matrices.append((off, s.numel // s.shape[-1], s.shape[-1]))
+            else:
+                self._vectors.append((off, s.numel))
+        if self._gpu:
+            self._nv._ns_steps(self._nv._ns_key(ns_coeffs), ns_steps)   # refuses coefficients here rather than in the first step
+            self._tables = self._nv.MuonTables(self._matrices, self._vectors, arena.params.device)
+
+    def step(self, lr: float, grad_scale: float = 1.0, vector_lr: Optional[float] = None) -> None:
+        """Updates every parameter from grads * grad_scale; vectors with step size `vector_lr` (default: lr)."""
+        a, t = self.arena, self.steps + 1
+        lr_t = (lr if vector_lr is None else vector_lr) * math.sqrt(1.0 - self.beta2 ** t) / (1.0 - self.beta1 ** t)
+        if self._gpu:
+            self._nv.set_scalars(self._hyper, (lr, self.momentum, grad_scale, 1.0 - lr * self.weight_decay, lr_t, 1.0 - self.beta1,
+                                               1.0 - self.beta2, self.eps))
+            self._nv.muon_step(a.params, a.grads, a.slots["m"], a.slots["v"], self._hyper, self._tables, nesterov=self.nesterov,
+                               steps=self.ns_steps, coeffs=self.ns_coeffs, eps=self.ns_eps)
+        else:
+            for off, rows, cols in self._matrices:
+                p, g, m = (b[off:off + rows * cols].view(rows, cols) for b in (a.params, a.grads, a.slots["m"]))
+                ref.muon_update(p, g * grad_scale, m, lr, self.momentum, self.nesterov, self.weight_decay, self.ns_steps, self.ns_coeffs, self.ns_eps)
+            for off, n in self._vectors:
+                p, g, m, v = (b[off:off + n] for b in (a.params, a.grads, a.slots["m"], a.slots["v"]))
+                ref.adam_update(p, g * grad_scale, m, v, lr_t, self.beta1, self.beta2, self.eps)
+        self.steps = t
