@@ -30,17 +30,27 @@ struct Plan {
 };
 Plan plan_of(const MmProduct& p) {
   Plan l{};
-  l.variant = LIN_REGS_128;
-  const int bm = kLinVariants[l.variant].bm, bn = kLinVariants[l.variant].bn;
-  const int kb = 128 / elem_bytes(p.kind);
-  l.gx = ceil_div(p.N, bn);
-  l.gy = ceil_div(p.M, bm);
+  const int es = elem_bytes(p.kind);
+  auto direct = [&](const void* base, long long ld, int contiguous) {
+    return aligned_to(base, 16) && !(ld * es & 15) && !((long long)contiguous * es & 15) && ld * es < (1 << 23);
+  };
+  const bool whole = direct(p.a, p.lda, p.kc_a ? p.K : p.M) && direct(p.b, p.ldb, p.kc_b ? p.K : p.N);
+  const long long tiles128 = (long long)ceil_div(p.M, 128) * ceil_div(p.N, 128), tiles256 = (long long)ceil_div(p.M, 256) * ceil_div(p.N, 256);
+  // The larger the tile the less it loads per product, as long as there is about a tile per CU (bf16, 256 / 128 / 64, us: 8192 x 4096 x 4096
+  // 224 / 298 / 383, 2048 cubed 39 / 23 / 28, 512 x 2048 x 2048 - / 17.1 / 14.5; fp32 2048 cubed 148 / 127 / 134).
+  l.variant = !whole ? LIN_REGS : tiles256 >= 192 ? LIN_256 : tiles128 >= 128 ? LIN_128 : LIN_64;
+  const int tile = kLinTiles[l.variant].t;
+  const int kb = 128 / es;
+  l.gx = ceil_div(p.N, tile);
+  l.gy = ceil_div(p.M, tile);
   l.N4 = ((long long)p.N + 3) / 4 * 4;
-  // Few tiles and a long k: several workgroups share a tile's k, at least four stages each, until every CU has one.
+  // Few tiles and a long k: several workgroups share a tile's k, at least eight stages each, until two stand on every CU
+  // (fp32 128 x 3136 x 512, 64 x 64 tiles, us in 1 / 4 / 8 / 16 parts: 40 / 22.4 / 19.0 / 18.8, the host's time).
   const long long tiles = (long long)l.gx * l.gy;
   const int stages = ceil_div(p.K, kb);
+  const int slots = l.variant == LIN_REGS || l.variant == LIN_64 ? 512 : 256;
   int splits = 1;
-  while (tiles * splits * 2 <= 512 && stages >= splits * 8 && (size_t)p.M * l.N4 * splits * 8 <= kMaxPartialBytes) splits *= 2;
+  while (tiles * splits * 2 <= slots && stages >= splits * 16 && (size_t)p.M * l.N4 * splits * 8 <= kMaxPartialBytes) splits *= 2;
   const int per = ceil_div(stages, splits) * kb;
   l.splits = p.K > 0 ? ceil_div(p.K, per) : 1;
   l.k_per_split = p.K > 0 ? per : kb;

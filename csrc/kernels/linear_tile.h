@@ -88,6 +88,14 @@ __device__ __forceinline__ void lin_finish(const MmProduct& p, int vec, int m, i
   lin_store4<KIND>(p.c, at, vec, have, v);
 }
 
+template <int NJ>
+struct LinEpilogue { static constexpr int PITCH = NJ * 16 + 4; };   // floats; the 16 bytes spread a column over the banks
+template <class Loop, int WAVES>
+constexpr int lin_lds() {
+  constexpr int epi = WAVES * 32 * LinEpilogue<Loop::NJ>::PITCH * 4;
+  return epi > Loop::LDS ? epi : Loop::LDS;
+}
+
 template <MmKind KIND, class Loop, int BM, int BN, int WGM, int WGN>
 __global__ __launch_bounds__(64 * WGM * WGN) void linear_tile_kernel(LinTileArgs a) {
   DTF_ABORT_GUARD(a);
@@ -109,18 +117,27 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tile_kernel(LinTileArgs
   const MmOperands o{reinterpret_cast<const char*>(p.a), reinterpret_cast<const char*>(p.b), p.lda, p.ldb, p.M, p.N};
   Loop::run(o, m0, n0, k_begin, k_end, lin_smem, acc);
 
+  // The sums leave through LDS, 32 rows of a wave's tile at a time: a loop over whole rows with 16 lanes to a row, so the
+  // tensors are read and written 64 columns at once and the epilogue's code exists once. Each wave has its own rows: no barrier.
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, l15 = lane & 15;
   const int wm = (wave / WGN) * (BM / WGM), wn = (wave % WGN) * (BN / WGN);
+  float* rows = reinterpret_cast<float*>(lin_smem) + wave * (32 * LinEpilogue<NJ>::PITCH);
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int m = m0 + wm + i * 16 + l15;
-    if (m >= p.M) continue;
+  for (int i0 = 0; i0 < MI; i0 += 2) {
+    if (m0 + wm + i0 * 16 >= p.M) break;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int n = n0 + wn + j * 16 + 4 * q;
-      if (n >= p.N) continue;
-      if (a.splits > 1) *reinterpret_cast<floatx4*>(a.partial + ((long long)split * p.M + m) * a.N4 + n) = acc[i][j];   // N4 covers the last n
-      else lin_finish<KIND>(p, a.vec, m, n, acc[i][j]);
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        *reinterpret_cast<floatx4*>(rows + (i * 16 + l15) * LinEpilogue<NJ>::PITCH + j * 16 + 4 * q) = acc[i0 + i][j];
+#pragma unroll 1
+    for (int e = lane; e < 32 * NJ * 4; e += 64) {
+      const int r = e / (NJ * 4), c = (e % (NJ * 4)) * 4;
+      const int m = m0 + wm + i0 * 16 + r, n = n0 + wn + c;
+      if (m >= p.M || n >= p.N) continue;
+      const floatx4 v = *reinterpret_cast<const floatx4*>(rows + r * LinEpilogue<NJ>::PITCH + c);
+      if (a.splits > 1) *reinterpret_cast<floatx4*>(a.partial + ((long long)split * p.M + m) * a.N4 + n) = v;   // N4 covers the last n
+      else lin_finish<KIND>(p, a.vec, m, n, v);
     }
   }
 }
@@ -209,19 +226,35 @@ const LinLaunch& lin_launch_f32();
 const LinLaunch& lin_launch_bf16();
 const LinLaunch& lin_launch_f16();
 
-enum LinVariant { LIN_REGS_128 = 0 };
-struct LinVariantInfo { int bm, bn; };
-constexpr LinVariantInfo kLinVariants[] = {{128, 128}};
+// The variants of the product kernel: tile, waves over it, stages in LDS, 128-byte pieces of k per stage.
+enum LinVariant { LIN_REGS = 0, LIN_64 = 1, LIN_128 = 2, LIN_256 = 3 };
+struct LinTile { int t, wgm, wgn, stages, subs; };
+constexpr LinTile kLinTiles[] = {{128, 2, 2, 1, 1}, {64, 2, 2, 4, 1}, {128, 2, 4, 2, 2}, {256, 2, 4, 2, 1}};
 
+template <MmKind KIND, bool KCA, bool KCB, int V>
+struct LinLoopOf {
+  static constexpr LinTile T = kLinTiles[V];
+  using type = MmDirect<KIND, KCA, KCB, T.t, T.t, T.wgm, T.wgn, true, T.stages, T.subs>;
+};
+template <MmKind KIND, bool KCA, bool KCB>
+struct LinLoopOf<KIND, KCA, KCB, LIN_REGS> {
+  using type = MmRegs<KIND, KCA, KCB, 128, 128, 2, 2, true>;
+};
+template <MmKind KIND, bool KCA, bool KCB, int V>
+void lin_tile_launch_as(const LinTileArgs& a, hipStream_t stream) {
+  constexpr LinTile T = kLinTiles[V];
+  constexpr int WAVES = T.wgm * T.wgn;
+  using Loop = typename LinLoopOf<KIND, KCA, KCB, V>::type;
+  launch("linear", linear_tile_kernel<KIND, Loop, T.t, T.t, T.wgm, T.wgn>, dim3((unsigned)((a.total + 7) / 8 * 8)), dim3(64 * WAVES), lin_lds<Loop, WAVES>(),
+         stream, a);
+}
 template <MmKind KIND, bool KCA, bool KCB>
 void lin_tile_launch(const LinTileArgs& a, int variant, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.total + 7) / 8 * 8));
   switch (variant) {
-    case LIN_REGS_128: {
-      using Loop = MmRegs<KIND, KCA, KCB, 128, 128, 2, 2, true>;
-      launch("linear", linear_tile_kernel<KIND, Loop, 128, 128, 2, 2>, grid, dim3(256), Loop::LDS, stream, a);
-      break;
-    }
+    case LIN_REGS: return lin_tile_launch_as<KIND, KCA, KCB, LIN_REGS>(a, stream);
+    case LIN_64: return lin_tile_launch_as<KIND, KCA, KCB, LIN_64>(a, stream);
+    case LIN_128: return lin_tile_launch_as<KIND, KCA, KCB, LIN_128>(a, stream);
+    case LIN_256: return lin_tile_launch_as<KIND, KCA, KCB, LIN_256>(a, stream);
     default: throw std::runtime_error("linear: unknown variant");
   }
 }

@@ -12,7 +12,7 @@
 namespace dtf {
 
 constexpr int kNsMaxSteps = 16;
-constexpr int kNsNormParts = 256;   // partial sums of a squared norm
+constexpr int kNsNormParts = 512;   // partial sums of a squared norm
 
 // One matrix. Its workspace (base `ws`, in floats from the call's workspace) holds
 //   [kNsNormParts doubles][tau, 63 spare][X, X': rp x cp pairs][A, P: rp x rp pairs]

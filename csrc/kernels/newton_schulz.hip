@@ -67,6 +67,30 @@ __device__ __forceinline__ double block_sum(double v, double* scratch) {
   return (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
 }
 
+__device__ __forceinline__ double squares(const uintx4& x, int kind) {
+  double s = 0.0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (kind == MM_F32) {
+      const double v = __uint_as_float(x[e]);
+      s += v * v;
+    } else {
+      float lo, hi;
+      if (kind == MM_BF16) {
+        lo = pair_lo(x[e]);
+        hi = pair_hi(x[e]);
+      } else {
+        const unsigned short a = (unsigned short)x[e], b = (unsigned short)(x[e] >> 16);
+        lo = (float)__builtin_bit_cast(_Float16, a);
+        hi = (float)__builtin_bit_cast(_Float16, b);
+      }
+      s += (double)lo * lo;
+      s += (double)hi * hi;
+    }
+  }
+  return s;
+}
+
 // Squares of one chunk of G, in 64 bits (squares of gradients leave fp32's range).
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsDev a) {
   __shared__ double scratch[4];
@@ -75,8 +99,25 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsDev a) {
   ns_find(a, blockIdx.x, m, chunk);
   const long long n = (long long)m.rows * m.cols;
   const long long lo = (long long)chunk * m.chunk, hi = min(n, lo + m.chunk);
+  const int es = a.kind == MM_F32 ? 4 : 2;
+  const char* base = reinterpret_cast<const char*>(a.g) + m.src * es;
   double s = 0.0;
-  for (long long i = lo + threadIdx.x; i < hi; i += 256) {
+  long long i = lo + threadIdx.x;
+  if (m.ld == m.cols && !(reinterpret_cast<uintptr_t>(base) & 15)) {
+    // whole rows back to back: 16 bytes a thread, four loads in flight (a chunk is a multiple of 64 elements)
+    const int epv = 16 / es;
+    const long long v0 = lo / epv, v1 = hi / epv;
+    const uintx4* src = reinterpret_cast<const uintx4*>(base);
+    for (long long v = v0 + threadIdx.x; v < v1; v += 1024) {
+      uintx4 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = v + 256 * u < v1 ? src[v + 256 * u] : uintx4{0, 0, 0, 0};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += squares(x[u], a.kind);
+    }
+    i = v1 * epv + threadIdx.x;
+  }
+  for (; i < hi; i += 256) {
     const long long row = i / m.cols;
     const float x = ns_read(a.g, a.kind, m.src + row * m.ld + (i - row * m.cols));
     s += (double)x * x;
@@ -157,7 +198,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsDev a) {
   ns_find(a, blockIdx.x, m, tile);
   float* base = a.ws + m.ws;
   const double* parts = reinterpret_cast<const double*>(base);
-  const double ss = block_sum((int)threadIdx.x < m.parts ? parts[threadIdx.x] : 0.0, scratch);
+  const double ss = block_sum(((int)threadIdx.x < m.parts ? parts[threadIdx.x] : 0.0) + ((int)threadIdx.x + 256 < m.parts ? parts[threadIdx.x + 256] : 0.0), scratch);
   const double norm = sqrt(ss), t = norm / (norm + a.eps);
   // tau: the power of two at or above t, 1 unless the norm is below eps (or is not a number)
   float tau = 1.f;
@@ -190,12 +231,23 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsDev a) {
 
 enum NsOp { NS_GRAM, NS_POLY, NS_APPLY };
 
+// Tiles: waves over T x T, stages in LDS, 128-byte pieces of k per stage; then what the choice between them goes by: workgroups
+// that the card holds at a time, and us per 32 of k of one round of them with half the CUs busy and with all (measured on 576 x 64 to
+// 4096 x 4096; us of a whole product by 64 / 128 / 192 / 256: X X^T of 1024 x 4096 36 / 73 / 133 / 216, of 4096 x 4096 322 / 246 / 175 / 221;
+// P X of 1024 x 4096 36 / 31 / 47 / 73, of 4096 x 4096 420 / 322 / 337 / 276).
+struct NsTileInfo { int t, wgm, wgn, stages, subs, slots; float us_some, us_full; };
+constexpr NsTileInfo kNsTiles[] = {{64, 2, 2, 4, 1, 512, 0.26f, 0.5f}, {128, 2, 4, 2, 2, 256, 0.57f, 0.8f}, {192, 2, 4, 2, 1, 256, 1.1f, 1.36f}, {256, 2, 4, 2, 1, 256, 1.7f, 2.15f}};
+template <int T>
+struct NsTile {
+  static constexpr NsTileInfo I = kNsTiles[T / 64 - 1];
+  static constexpr int WGM = I.wgm, WGN = I.wgn, STAGES = I.stages, SUBS = I.subs, NT = 64 * WGM * WGN;
+};
 template <int T, bool KCB, bool SWAP>
-using NsLoop = MmRegs<MM_PAIR, true, KCB, T, T, 2, 2, SWAP>;
+using NsLoop = MmDirect<MM_PAIR, true, KCB, T, T, NsTile<T>::WGM, NsTile<T>::WGN, SWAP, NsTile<T>::STAGES, NsTile<T>::SUBS>;
 
 // One T x T tile of one of the three products.
 template <NsOp OP, int T>
-__global__ __launch_bounds__(256) void ns_product_kernel(NsDev a) {
+__global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
   extern __shared__ __attribute__((aligned(16))) char ns_smem[];
   const int t = mm_item(blockIdx.x, a.total);
   if (t >= a.total) return;
@@ -216,14 +268,14 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsDev a) {
   if (a.step & 1) { float* s = xa; xa = xb; xb = s; }
   float *A = a.ws + ns_a(m), *P = a.ws + ns_p(m);
 
-  constexpr int MI = T / 32, NJ = T / 32;
+  constexpr int WGM = NsTile<T>::WGM, WGN = NsTile<T>::WGN, MI = T / WGM / 16, NJ = T / WGN / 16;
   floatx4 acc[MI][NJ];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, l15 = lane & 15;
-  const int wm = (wave >> 1) * (T / 2), wn = (wave & 1) * (T / 2);
+  const int wm = (wave / WGN) * (T / WGM), wn = (wave % WGN) * (T / WGN);
 
   if (OP != NS_APPLY) {
     const float* src = OP == NS_GRAM ? xa : A;
@@ -320,11 +372,25 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsDev a) {
 template <NsOp OP>
 void product(const char* name, NsDev d, int tile, hipStream_t stream) {
   const dim3 grid((unsigned)((d.total + 7) / 8 * 8));
-  if (tile == 128) launch(name, ns_product_kernel<OP, 128>, grid, dim3(256), NsLoop<128, true, true>::LDS, stream, d);
-  else launch(name, ns_product_kernel<OP, 64>, grid, dim3(256), NsLoop<64, true, true>::LDS, stream, d);
+  if (tile == 256) launch(name, ns_product_kernel<OP, 256>, grid, dim3(512), NsLoop<256, true, true>::LDS, stream, d);
+  else if (tile == 192) launch(name, ns_product_kernel<OP, 192>, grid, dim3(512), NsLoop<192, true, true>::LDS, stream, d);
+  else if (tile == 128) launch(name, ns_product_kernel<OP, 128>, grid, dim3(NsTile<128>::NT), NsLoop<128, true, true>::LDS, stream, d);
+  else launch(name, ns_product_kernel<OP, 64>, grid, dim3(NsTile<64>::NT), NsLoop<64, true, true>::LDS, stream, d);
 }
 
 int sym_tiles(const NsMat& m, int T) { const int t = ceil_div(m.rp, T); return t * (t + 1) / 2; }
+// The tile with the least estimated time: rounds of workgroups times k.
+template <class Count>
+int pick_tile(Count&& count, int k_stages) {
+  int best = 64;
+  float least = 0.f;
+  for (const NsTileInfo& i : kNsTiles) {
+    const long long n = count(i.t);
+    const float us = (float)k_stages * (float)((n + i.slots - 1) / i.slots) * (n <= 160 ? i.us_some : i.us_full);
+    if (i.t == 64 || us < least) { best = i.t; least = us; }
+  }
+  return best;
+}
 int apply_tiles(const NsMat& m, int T) { return ceil_div(m.rp, T) * ceil_div(m.cp, T); }
 
 }  // namespace
@@ -338,7 +404,7 @@ void ns_shape(NsMat& m, int rows, int cols) {
   m.cp = ceil_div(m.c, 32) * 32;
   const long long n = (long long)rows * cols;
   const long long chunk = (n + kNsNormParts - 1) / kNsNormParts;
-  m.chunk = (int)(chunk < 2048 ? 2048 : chunk);
+  m.chunk = (int)(((chunk < 2048 ? 2048 : chunk) + 63) / 64 * 64);
   m.parts = (int)((n + m.chunk - 1) / m.chunk);
   float s = 1.f;
   while (s * s < (float)n && s < 8192.f) s *= 2.f;   // the iterates stay below 3.8: 3.8 * 8192 is inside fp16's range
@@ -374,14 +440,16 @@ void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t strea
   launch("ns_norm", ns_norm_kernel, dim3(n.total), dim3(256), 0, stream, n);
   const NsDev s = with((m.rp / 32) * (m.cp / 32));
   launch("ns_split", ns_split_kernel, dim3(s.total), dim3(256), 0, stream, s);
-  const int tile = (long long)apply_tiles(m, 128) * a.batch >= 128 ? 128 : 64;
+  const int tg = pick_tile([&](int T) { return (long long)sym_tiles(m, T) * a.batch; }, m.cp / 32);
+  const int tp = pick_tile([&](int T) { return (long long)sym_tiles(m, T) * a.batch; }, m.rp / 32);
+  const int ta = pick_tile([&](int T) { return (long long)apply_tiles(m, T) * a.batch; }, m.rp / 32);
   for (int k = 0; k < a.steps; ++k) {
     d.step = k;
     d.last = k == a.steps - 1;
     d.co = a.coeffs[k];
-    product<NS_GRAM>("ns_gram", with(sym_tiles(m, tile)), tile, stream);
-    product<NS_POLY>("ns_poly", with(sym_tiles(m, tile)), tile, stream);
-    product<NS_APPLY>("ns_apply", with(apply_tiles(m, tile)), tile, stream);
+    product<NS_GRAM>("ns_gram", with(sym_tiles(m, tg)), tg, stream);
+    product<NS_POLY>("ns_poly", with(sym_tiles(m, tp)), tp, stream);
+    product<NS_APPLY>("ns_apply", with(apply_tiles(m, ta)), ta, stream);
   }
 }
 
