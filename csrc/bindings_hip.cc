@@ -484,7 +484,7 @@ PYBIND11_MODULE(_hip, m) {
   // Dense layers: positional, since a single-row call costs no more than its Python call does. An address is 0 for a
   // tensor that is left out; the workspace query takes the same arguments.
   {
-    auto fwd = [](int kind, int M, int N, int K, int trans_w, int act, uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t bias,
+    auto fwd = [](int kind, int M, int N, int K, bool trans_w, int act, uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t bias,
                   uint64_t res, long long ldr, uint64_t y, long long ldy, uint64_t pre, long long ldp) {
       LinearArgs a{};
       a.kind = kind; a.M = M; a.N = N; a.K = K; a.trans_w = trans_w; a.act = act;
@@ -493,17 +493,17 @@ PYBIND11_MODULE(_hip, m) {
       a.y = reinterpret_cast<void*>(y); a.ldy = ldy; a.pre = reinterpret_cast<void*>(pre); a.ldp = ldp;
       return a;
     };
-    m.def("linear_workspace", [fwd](int kind, int M, int N, int K, int trans_w, int act, uint64_t x, long long ldx, uint64_t w, long long ldw,
+    m.def("linear_workspace", [fwd](int kind, int M, int N, int K, bool trans_w, int act, uint64_t x, long long ldx, uint64_t w, long long ldw,
                                     uint64_t bias, uint64_t res, long long ldr, uint64_t y, long long ldy, uint64_t pre, long long ldp) {
       return linear_workspace(fwd(kind, M, N, K, trans_w, act, x, ldx, w, ldw, bias, res, ldr, y, ldy, pre, ldp));
     });
-    m.def("linear", [fwd](int kind, int M, int N, int K, int trans_w, int act, uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t bias,
+    m.def("linear", [fwd](int kind, int M, int N, int K, bool trans_w, int act, uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t bias,
                           uint64_t res, long long ldr, uint64_t y, long long ldy, uint64_t pre, long long ldp, uint64_t ws, size_t ws_bytes,
                           uint64_t stream) {
       linear(fwd(kind, M, N, K, trans_w, act, x, ldx, w, ldw, bias, res, ldr, y, ldy, pre, ldp), reinterpret_cast<void*>(ws), ws_bytes,
              as_stream(stream));
     });
-    auto bwd = [](int kind, int M, int N, int K, int trans_w, int act, int accumulate, uint64_t dy, long long lddy, uint64_t pre, long long ldp,
+    auto bwd = [](int kind, int M, int N, int K, bool trans_w, int act, bool accumulate, uint64_t dy, long long lddy, uint64_t pre, long long ldp,
                   uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t dx, long long lddx, uint64_t dw, long long lddw, uint64_t db) {
       LinearBwdArgs a{};
       a.kind = kind; a.M = M; a.N = N; a.K = K; a.trans_w = trans_w; a.act = act; a.accumulate = accumulate;
@@ -513,12 +513,12 @@ PYBIND11_MODULE(_hip, m) {
       a.db = reinterpret_cast<void*>(db);
       return a;
     };
-    m.def("linear_bwd_workspace", [bwd](int kind, int M, int N, int K, int trans_w, int act, int accumulate, uint64_t dy, long long lddy, uint64_t pre,
+    m.def("linear_bwd_workspace", [bwd](int kind, int M, int N, int K, bool trans_w, int act, bool accumulate, uint64_t dy, long long lddy, uint64_t pre,
                                         long long ldp, uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t dx, long long lddx, uint64_t dw,
                                         long long lddw, uint64_t db) {
       return linear_bwd_workspace(bwd(kind, M, N, K, trans_w, act, accumulate, dy, lddy, pre, ldp, x, ldx, w, ldw, dx, lddx, dw, lddw, db));
     });
-    m.def("linear_bwd", [bwd](int kind, int M, int N, int K, int trans_w, int act, int accumulate, uint64_t dy, long long lddy, uint64_t pre,
+    m.def("linear_bwd", [bwd](int kind, int M, int N, int K, bool trans_w, int act, bool accumulate, uint64_t dy, long long lddy, uint64_t pre,
                               long long ldp, uint64_t x, long long ldx, uint64_t w, long long ldw, uint64_t dx, long long lddx, uint64_t dw,
                               long long lddw, uint64_t db, uint64_t ws, size_t ws_bytes, uint64_t stream) {
       linear_bwd(bwd(kind, M, N, K, trans_w, act, accumulate, dy, lddy, pre, ldp, x, ldx, w, ldw, dx, lddx, dw, lddw, db),

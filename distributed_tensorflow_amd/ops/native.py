@@ -1032,17 +1032,20 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _mat(t: torch.Tensor, what: str, like: torch.Tensor, shape, written: bool = False) -> tuple:
-    """(address, row stride in elements) of a row-strided matrix; shape entries of None are free."""
-    if t.dim() != 2 or any(w is not None and s != w for s, w in zip(t.shape, shape)):
-        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+def _mat(t: torch.Tensor, what: str, like: torch.Tensor, rows: int, cols: int, written: bool = False) -> tuple:
+    """(address, row stride in elements) of a row-strided matrix; a size of -1 is free."""
+    shape = t.shape
+    if len(shape) != 2 or (shape[0] != rows and rows >= 0) or (shape[1] != cols and cols >= 0):
+        raise ValueError(f"{what}: expected shape {[rows, cols]}, got {list(shape)}")
+    rows, cols = shape
     if t.dtype != like.dtype:
         raise ValueError(f"{what}: expected {like.dtype}, got {t.dtype}")
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise ValueError(f"{what}: on {t.device}, expected {like.device}")
-    rows, cols = t.shape
-    ld = t.stride(0) if rows > 1 else cols
-    if cols > 1 and t.stride(1) != 1:
+    ld, step = t.stride()
+    if rows <= 1:
+        ld = cols
+    if step != 1 and cols > 1:
         raise ValueError(f"{what}: the elements of a row must be contiguous")
     if written and ld < cols:
         raise ValueError(f"{what}: rows overlap")
@@ -1051,14 +1054,26 @@ def _mat(t: torch.Tensor, what: str, like: torch.Tensor, shape, written: bool = 
     return t.data_ptr(), ld
 
 
-def _check_device(t: torch.Tensor, what: str) -> None:
+_have_gpu = False
+
+
+def _check_device(t: torch.Tensor, what: str) -> int:
+    """The tensors' device index, which has to be the current one."""
+    global _have_gpu
     if t.dtype not in _KINDS:
         raise ValueError(f"{what}: float32, bfloat16 or float16 tensors, got {t.dtype}")
-    require()
-    if not t.is_cuda:
+    if not _have_gpu:
+        require()
+        _have_gpu = True
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError(f"{what}: expected GPU tensors")
-    if t.get_device() != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         raise ValueError(f"{what}: the tensors are on {t.device}, the current device is {torch.cuda.current_device()}")
+    return dev
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the current stream's handle without a Stream object around it
 
 
 def _span(t: torch.Tensor) -> tuple:
@@ -1113,30 +1128,36 @@ def linear(x, w, bias=None, *, activation: str = "none", residual=None, trans_w:
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"linear: unknown activation {activation!r}")
-    px, ldx = _mat(x, "linear: x", x, (None, None))
+    px, ldx = _mat(x, "linear: x", x, -1, -1)
     m, k = x.shape
-    pw, ldw = _mat(w, "linear: w", x, (None, k) if trans_w else (k, None))
+    pw, ldw = _mat(w, "linear: w", x, -1, k) if trans_w else _mat(w, "linear: w", x, k, -1)
     n = w.shape[0] if trans_w else w.shape[1]
     pb = pr = pp = ldr = ldp = 0
     if bias is not None:
-        if tuple(bias.shape) != (n,) or bias.dtype != x.dtype or bias.device != x.device or (n > 1 and bias.stride(0) != 1):
+        if bias.dim() != 1 or bias.shape[0] != n or bias.dtype != x.dtype or bias.get_device() != x.get_device() or (n > 1 and bias.stride(0) != 1):
             raise ValueError(f"linear: bias must be a contiguous {x.dtype} vector of {n} on {x.device}")
         pb = bias.data_ptr()
     if residual is not None:
-        pr, ldr = _mat(residual, "linear: residual", x, (m, n))
+        pr, ldr = _mat(residual, "linear: residual", x, m, n)
     if out is None:
-        out = torch.empty((m, n), device=x.device, dtype=x.dtype)
         if pre is not None:
             _check_apart("linear", (pre,), (x, w, bias, residual))
     else:
         _check_apart("linear", (out, pre), (x, w, bias), (residual,))
-    py, ldy = _mat(out, "linear: out", x, (m, n), written=True)
+        py, ldy = _mat(out, "linear: out", x, m, n, written=True)
     if pre is not None:
-        pp, ldp = _mat(pre, "linear: pre", x, (m, n), written=True)
-    _check_device(x, "linear")
-    args = (_KINDS[x.dtype], m, n, k, int(trans_w), act, px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pp, ldp)
-    ws, addr, have = _workspace("linear", _hip.linear_workspace(*args), workspace, x.device)
-    _hip.linear(*args, addr, have, stream())
+        pp, ldp = _mat(pre, "linear: pre", x, m, n, written=True)
+    dev = _check_device(x, "linear")
+    if out is None:
+        out = torch.empty((m, n), device=x.device, dtype=x.dtype)
+        py, ldy = out.data_ptr(), n
+    args = (_KINDS[x.dtype], m, n, k, trans_w, act, px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pp, ldp)
+    need = _hip.linear_workspace(*args)
+    if need or workspace is not None:
+        ws, addr, have = _workspace("linear", need, workspace, x.device)
+        _hip.linear(*args, addr, have, _raw_stream(dev))
+    else:
+        _hip.linear(*args, 0, 0, _raw_stream(dev))
     return out
 
 
@@ -1151,17 +1172,17 @@ def linear_bwd(dy, x, w, *, pre=None, activation: str = "none", trans_w: bool = 
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"linear_bwd: unknown activation {activation!r}")
-    pdy, lddy = _mat(dy, "linear_bwd: dy", dy, (None, None))
+    pdy, lddy = _mat(dy, "linear_bwd: dy", dy, -1, -1)
     m, n = dy.shape
-    px, ldx = _mat(x, "linear_bwd: x", dy, (m, None))
+    px, ldx = _mat(x, "linear_bwd: x", dy, m, -1)
     k = x.shape[1]
     wshape = (n, k) if trans_w else (k, n)
-    pw, ldw = _mat(w, "linear_bwd: w", dy, wshape)
+    pw, ldw = _mat(w, "linear_bwd: w", dy, *wshape)
     pp = ldp = 0
     if act:
         if pre is None:
             raise ValueError("linear_bwd: the gradient of an activation needs pre")
-        pp, ldp = _mat(pre, "linear_bwd: pre", dy, (m, n))
+        pp, ldp = _mat(pre, "linear_bwd: pre", dy, m, n)
     if accumulate and (dw is True or db is True):
         raise ValueError("linear_bwd: accumulate=True adds to tensors that are given")
     given = [t for t in (dx, dw, db) if isinstance(t, torch.Tensor)]
@@ -1174,17 +1195,17 @@ def linear_bwd(dy, x, w, *, pre=None, activation: str = "none", trans_w: bool = 
         return t if isinstance(t, torch.Tensor) else None
 
     dx, dw, db = output(dx, (m, k)), output(dw, wshape), output(db, (n,))
-    pdx, lddx = _mat(dx, "linear_bwd: dx", dy, (m, k), written=True) if dx is not None else (0, 0)
-    pdw, lddw = _mat(dw, "linear_bwd: dw", dy, wshape, written=True) if dw is not None else (0, 0)
+    pdx, lddx = _mat(dx, "linear_bwd: dx", dy, m, k, written=True) if dx is not None else (0, 0)
+    pdw, lddw = _mat(dw, "linear_bwd: dw", dy, *wshape, written=True) if dw is not None else (0, 0)
     pdb = 0
     if db is not None:
-        if tuple(db.shape) != (n,) or db.dtype != dy.dtype or db.device != dy.device or (n > 1 and db.stride(0) != 1):
+        if db.dim() != 1 or db.shape[0] != n or db.dtype != dy.dtype or db.get_device() != dy.get_device() or (n > 1 and db.stride(0) != 1):
             raise ValueError(f"linear_bwd: db must be a contiguous {dy.dtype} vector of {n} on {dy.device}")
         pdb = db.data_ptr()
-    _check_device(dy, "linear_bwd")
-    args = (_KINDS[dy.dtype], m, n, k, int(trans_w), act, int(accumulate), pdy, lddy, pp, ldp, px, ldx, pw, ldw, pdx, lddx, pdw, lddw, pdb)
+    dev = _check_device(dy, "linear_bwd")
+    args = (_KINDS[dy.dtype], m, n, k, trans_w, act, accumulate, pdy, lddy, pp, ldp, px, ldx, pw, ldw, pdx, lddx, pdw, lddw, pdb)
     ws, addr, have = _workspace("linear_bwd", _hip.linear_bwd_workspace(*args), workspace, dy.device)
-    _hip.linear_bwd(*args, addr, have, stream())
+    _hip.linear_bwd(*args, addr, have, _raw_stream(dev))
     return dx, dw, db
 
 
@@ -1240,7 +1261,7 @@ def newton_schulz(g, *, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out
     rows, cols = g.shape[-2:]
 
     def place(t, what, written):
-        _mat(t if t.dim() == 2 else t[0] if t.shape[0] else t.new_empty(rows, cols), what, g, (rows, cols), written)
+        _mat(t if t.dim() == 2 else t[0] if t.shape[0] else t.new_empty(rows, cols), what, g, rows, cols, written)
         ld, gap = (t.stride(-2) if rows > 1 else cols), (t.stride(0) if t.dim() == 3 and t.shape[0] > 1 else 0)
         if written and t.dim() == 3 and t.shape[0] > 1 and not (gap >= ld * (rows - 1) + cols or (gap >= cols and ld >= gap * (t.shape[0] - 1) + cols)):
             raise ValueError(f"{what}: the matrices overlap")
@@ -1252,13 +1273,13 @@ def newton_schulz(g, *, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out
     elif out.shape != g.shape:
         raise ValueError(f"newton_schulz: out has shape {tuple(out.shape)}, expected {tuple(g.shape)}")
     po = place(out, "newton_schulz: out", True)
-    _check_device(g, "newton_schulz")
+    dev = _check_device(g, "newton_schulz")
     if g.numel() == 0:
         return out
     batch = g.shape[0] if g.dim() == 3 else 1
     kind = _KINDS[g.dtype]
     ws, addr, have = _workspace("newton_schulz", _hip.newton_schulz_workspace(kind, batch, rows, cols), workspace, g.device)
-    _hip.newton_schulz(kind, batch, rows, cols, *pg, *po, eps, flat, growth, addr, have, stream())
+    _hip.newton_schulz(kind, batch, rows, cols, *pg, *po, eps, flat, growth, addr, have, _raw_stream(dev))
     return out
 
 
