@@ -9,6 +9,9 @@
 namespace dtf {
 namespace {
 
+// Rows that the few-rows kernels take. More go through 64 x 64 tiles: 4096 x 4096, us by rows kernel / tiles, bf16 W [K,N] 1 row
+// 10.3 / 17, 4 rows 13.3 / 13.7, 8 rows (spills) 37 / 13.7; fp32 8 rows 18.3 / 25.9.
+constexpr int lin_rows_max(int kind) { return kind == MM_F32 ? 8 : 4; }
 constexpr size_t kMaxPartialBytes = 256ull << 20;   // partial sums of a split product
 
 const LinLaunch& lin_launch(int kind) {
@@ -39,8 +42,22 @@ Plan plan_of(const MmProduct& p) {
   // The larger the tile the less it loads per product, as long as there is about a tile per CU (bf16, 256 / 128 / 64, us: 8192 x 4096 x 4096
   // 224 / 298 / 383, 2048 cubed 39 / 23 / 28, 512 x 2048 x 2048 - / 17.1 / 14.5; fp32 2048 cubed 148 / 127 / 134).
   l.variant = !whole ? LIN_REGS : tiles256 >= 192 ? LIN_256 : tiles128 >= 128 ? LIN_128 : LIN_64;
-  const int tile = kLinTiles[l.variant].t;
   const int kb = 128 / es;
+  // A few rows: no tile is worth filling. x has to fit LDS where W's rows are along k.
+  if (whole && p.kc_a && p.M <= lin_rows_max(p.kind) && !(p.K & 7) && p.K > 0 && (!p.kc_b || (long long)8 * p.K * es <= 128 * 1024)) {
+    l.variant = LIN_ROWS;
+    l.N4 = ((long long)p.N + 3) / 4 * 4;
+    l.gx = p.kc_b ? ceil_div(p.N, kRowWaves) : ceil_div(p.N, lin_row_lanes(p.N, 16 / es) * (16 / es));
+    l.gy = 1;
+    // W [K,N] with few columns: workgroups along k, where one would read more than 256 KB (a second launch costs what it reads in that time)
+    int splits = 1;
+    if (!p.kc_b) while (l.gx * splits * 2 <= 256 && (long long)p.K * 64 / splits >= 256 * 1024) splits *= 2;
+    l.k_per_split = ceil_div(ceil_div(p.K, splits), 8) * 8;
+    l.splits = ceil_div(p.K, l.k_per_split);
+    l.bytes = l.splits > 1 ? round_up((size_t)l.splits * p.M * l.N4 * sizeof(float)) : 0;
+    return l;
+  }
+  const int tile = kLinTiles[l.variant].t;
   l.gx = ceil_div(p.N, tile);
   l.gy = ceil_div(p.M, tile);
   l.N4 = ((long long)p.N + 3) / 4 * 4;

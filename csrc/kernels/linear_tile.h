@@ -16,26 +16,54 @@ struct LinTileArgs {
   AbortRef abort;
 };
 
+// Exponential and logistic function: the library's for fp32 tensors; for 16-bit ones, which round to 2^-9 and 2^-12, the hardware's
+// base-2 exponential and reciprocal (a few 2^-23 relative for the arguments that matter).
+template <MmKind KIND>
+__device__ __forceinline__ float lin_exp(float x) {
+  return KIND == MM_F32 ? expf(x) : __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
+}
+template <MmKind KIND>
+__device__ __forceinline__ float lin_logistic(float x) {
+  const float d = 1.f + lin_exp<KIND>(-x);
+  return KIND == MM_F32 ? 1.f / d : __builtin_amdgcn_rcpf(d);
+}
+// Phi(z), the normal distribution function, and e^(-z^2/2). 16-bit tensors: erfc(x) = (a1 t + ... + a5 t^5) e^(-x^2), t = 1 / (1 + p x), off by
+// at most 1.5e-7 (Abramowitz and Stegun, 7.1.26) - erff and the like cost 35 us of the 450 of an 8192 x 4096 x 8192 product.
+template <MmKind KIND>
+__device__ __forceinline__ float lin_phi(float z, float& gauss) {
+  gauss = lin_exp<KIND>(-0.5f * z * z);
+  if (KIND == MM_F32) return 0.5f * (1.f + erff(z * 0.70710678118654752f));
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678118654752f * fabsf(z));
+  const float tail = 0.5f * gauss * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  return z < 0.f ? tail : 1.f - tail;
+}
 // A value before the activation -> act(z). NaN stays NaN.
+template <MmKind KIND>
 __device__ __forceinline__ float lin_act(int act, float z) {
+  float gauss;
   switch (act) {
     case ACT_RELU: return z < 0.f ? 0.f : z;
-    case ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case ACT_GELU_TANH: return z / (1.f + expf(-1.5957691216057308f * (z + 0.044715f * z * z * z)));   // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
-    case ACT_SILU: return z / (1.f + expf(-z));
+    case ACT_GELU: return z * lin_phi<KIND>(z, gauss);
+    case ACT_GELU_TANH: return z * lin_logistic<KIND>(1.5957691216057308f * (z + 0.044715f * z * z * z));   // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
+    case ACT_SILU: return z * lin_logistic<KIND>(z);
     default: return z;
   }
 }
+template <MmKind KIND>
 __device__ __forceinline__ float lin_act_grad(int act, float z) {
+  float gauss;
   switch (act) {
     case ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+    case ACT_GELU: {
+      const float phi = lin_phi<KIND>(z, gauss);
+      return phi + z * gauss * 0.39894228040143268f;
+    }
     case ACT_GELU_TANH: {
-      const float q = 1.f / (1.f + expf(-1.5957691216057308f * (z + 0.044715f * z * z * z)));
+      const float q = lin_logistic<KIND>(1.5957691216057308f * (z + 0.044715f * z * z * z));
       return q + z * q * (1.f - q) * (1.5957691216057308f * (1.f + 0.134145f * z * z));
     }
     case ACT_SILU: {
-      const float q = 1.f / (1.f + expf(-z));
+      const float q = lin_logistic<KIND>(z);
       return q * (1.f + z * (1.f - q));
     }
     default: return 1.f;
@@ -72,20 +100,37 @@ __device__ __forceinline__ void lin_store4(void* base, long long at, int vec, in
   }
 }
 
-// The epilogue of four consecutive n of row m: every tensor is rounded once, from the fp32 value.
+// The epilogue of four consecutive n of row m: every tensor is rounded once, from the fp32 value. What it reads comes apart, so that
+// a caller can have several rows' reads in flight.
 template <MmKind KIND>
-__device__ __forceinline__ void lin_finish(const MmProduct& p, int vec, int m, int n, floatx4 v) {
+struct LinRead { floatx4 res, old; };
+template <MmKind KIND>
+__device__ __forceinline__ LinRead<KIND> lin_read(const MmProduct& p, int vec, int m, int n) {
+  LinRead<KIND> r;
+  if (p.res) r.res = lin_load4<KIND>(p.res, (long long)m * p.ldr + n, vec, p.N - n);
+  if (p.accumulate) r.old = lin_load4<KIND>(p.c, (long long)m * p.ldc + n, vec, p.N - n);
+  return r;
+}
+template <MmKind KIND>
+__device__ __forceinline__ void lin_finish(const MmProduct& p, int vec, int m, int n, floatx4 v, const floatx4& bias, const LinRead<KIND>& r) {
   const int have = p.N - n;
-  if (p.bias) v += lin_load4<KIND>(p.bias, n, vec, have);
+  v += bias;
   if (p.pre) lin_store4<KIND>(p.pre, (long long)m * p.ldp + n, vec, have, v);
   if (p.act != ACT_NONE) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = lin_act(p.act, v[i]);
+    for (int i = 0; i < 4; ++i) v[i] = lin_act<KIND>(p.act, v[i]);
   }
-  if (p.res) v += lin_load4<KIND>(p.res, (long long)m * p.ldr + n, vec, have);
-  const long long at = (long long)m * p.ldc + n;
-  if (p.accumulate) v += lin_load4<KIND>(p.c, at, vec, have);
-  lin_store4<KIND>(p.c, at, vec, have, v);
+  if (p.res) v += r.res;
+  if (p.accumulate) v += r.old;
+  lin_store4<KIND>(p.c, (long long)m * p.ldc + n, vec, have, v);
+}
+template <MmKind KIND>
+__device__ __forceinline__ floatx4 lin_bias(const MmProduct& p, int vec, int n) {
+  return p.bias ? lin_load4<KIND>(p.bias, n, vec, p.N - n) : floatx4{0.f, 0.f, 0.f, 0.f};
+}
+template <MmKind KIND>
+__device__ __forceinline__ void lin_finish(const MmProduct& p, int vec, int m, int n, const floatx4& v) {
+  lin_finish<KIND>(p, vec, m, n, v, lin_bias<KIND>(p, vec, n), lin_read<KIND>(p, vec, m, n));
 }
 
 template <int NJ>
@@ -121,23 +166,39 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tile_kernel(LinTileArgs
   // tensors are read and written 64 columns at once and the epilogue's code exists once. Each wave has its own rows: no barrier.
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, l15 = lane & 15;
   const int wm = (wave / WGN) * (BM / WGM), wn = (wave % WGN) * (BN / WGN);
-  float* rows = reinterpret_cast<float*>(lin_smem) + wave * (32 * LinEpilogue<NJ>::PITCH);
+  constexpr int PITCH = LinEpilogue<NJ>::PITCH, LANES = NJ * 4, RSTEP = 64 / LANES, U = 4;   // lanes to a row, rows at once, reads ahead
+  static_assert(64 % LANES == 0 && 32 % (RSTEP * U) == 0, "a lane keeps its columns");
+  float* rows = reinterpret_cast<float*>(lin_smem) + wave * (32 * PITCH);
+  const int c = (lane % LANES) * 4, n = n0 + wn + c, r0 = lane / LANES;
+  floatx4 bias = {0.f, 0.f, 0.f, 0.f};
+  if (a.splits == 1 && n < p.N) bias = lin_bias<KIND>(p, a.vec, n);
 #pragma unroll
   for (int i0 = 0; i0 < MI; i0 += 2) {
-    if (m0 + wm + i0 * 16 >= p.M) break;
+    const int mb = m0 + wm + i0 * 16;
+    if (mb >= p.M) break;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        *reinterpret_cast<floatx4*>(rows + (i * 16 + l15) * LinEpilogue<NJ>::PITCH + j * 16 + 4 * q) = acc[i0 + i][j];
+      for (int j = 0; j < NJ; ++j) *reinterpret_cast<floatx4*>(rows + (i * 16 + l15) * PITCH + j * 16 + 4 * q) = acc[i0 + i][j];
+    if (n >= p.N) continue;
 #pragma unroll 1
-    for (int e = lane; e < 32 * NJ * 4; e += 64) {
-      const int r = e / (NJ * 4), c = (e % (NJ * 4)) * 4;
-      const int m = m0 + wm + i0 * 16 + r, n = n0 + wn + c;
-      if (m >= p.M || n >= p.N) continue;
-      const floatx4 v = *reinterpret_cast<const floatx4*>(rows + r * LinEpilogue<NJ>::PITCH + c);
-      if (a.splits > 1) *reinterpret_cast<floatx4*>(a.partial + ((long long)split * p.M + m) * a.N4 + n) = v;   // N4 covers the last n
-      else lin_finish<KIND>(p, a.vec, m, n, v);
+    for (int r = r0; r < 32; r += RSTEP * U) {
+      if (a.splits > 1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (mb + r + u * RSTEP < p.M)   // N4 covers the last n
+            *reinterpret_cast<floatx4*>(a.partial + ((long long)split * p.M + mb + r + u * RSTEP) * a.N4 + n) =
+                *reinterpret_cast<const floatx4*>(rows + (r + u * RSTEP) * PITCH + c);
+        continue;
+      }
+      LinRead<KIND> rd[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (mb + r + u * RSTEP < p.M) rd[u] = lin_read<KIND>(p, a.vec, mb + r + u * RSTEP, n);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (mb + r + u * RSTEP < p.M)
+          lin_finish<KIND>(p, a.vec, mb + r + u * RSTEP, n, *reinterpret_cast<const floatx4*>(rows + (r + u * RSTEP) * PITCH + c), bias, rd[u]);
     }
   }
 }
@@ -154,6 +215,161 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinTileArgs a) {
     for (int s = 1; s < a.splits; ++s) v += *reinterpret_cast<const floatx4*>(src + s * plane);
     const int m = (int)(i / per_row), n = (int)(i - m * per_row) * 4;
     lin_finish<KIND>(a.p, a.vec, m, n, v);
+  }
+}
+
+// ---- A few rows: the weights are read once and that is all the time there is. 16 waves a workgroup, as many 16-byte
+// loads in flight as a wave has use for, fp32 multiply-adds on the vector pipe, sums in a fixed order.
+constexpr int kRowWaves = 16;
+template <MmKind KIND>
+__device__ __forceinline__ void row_unpack(const uintx4& v, float (&f)[16 / sizeof(typename MmElem<KIND>::type)]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (KIND == MM_F32) {
+      f[i] = __uint_as_float(v[i]);
+    } else if constexpr (KIND == MM_BF16) {
+      f[2 * i] = pair_lo(v[i]);
+      f[2 * i + 1] = pair_hi(v[i]);
+    } else {
+      f[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)v[i]);
+      f[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(v[i] >> 16));
+    }
+  }
+}
+// Sums of a workgroup's waves: part[wave][m][cols] -> the epilogue, or the split's partial sums.
+template <MmKind KIND, int MR>
+__device__ __forceinline__ void row_finish(const LinTileArgs& a, const float* part, int cols, int n0, int split) {
+  __syncthreads();
+  const int per_row = cols / 4;
+  for (int e = threadIdx.x; e < MR * per_row; e += 64 * kRowWaves) {
+    const int m = e / per_row, c = (e - m * per_row) * 4, n = n0 + c;
+    if (m >= a.p.M || n >= a.p.N) continue;
+    floatx4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) v += *reinterpret_cast<const floatx4*>(part + (w * MR + m) * cols + c);
+    if (a.splits > 1) *reinterpret_cast<floatx4*>(a.partial + ((long long)split * a.p.M + m) * a.N4 + n) = v;
+    else lin_finish<KIND>(a.p, a.vec, m, n, v);
+  }
+}
+// W [K,N]: a lane owns one 16-byte chunk of columns and eight consecutive k; LPR lanes side by side make the columns of a
+// workgroup, the 64 / LPR others go along k.
+template <MmKind KIND, int MR, int LPR>
+__global__ __launch_bounds__(64 * kRowWaves) void linear_row_n_kernel(LinTileArgs a) {
+  DTF_ABORT_GUARD(a);
+  using E = typename MmElem<KIND>::type;
+  constexpr int EPC = 16 / sizeof(E), COLS = LPR * EPC, KL = 64 / LPR;   // lanes along k
+  extern __shared__ __attribute__((aligned(16))) char lin_smem[];
+  float* part = reinterpret_cast<float*>(lin_smem);
+  const int t = mm_item(blockIdx.x, a.total);   // neighbours in n, which share cache lines, on one XCD
+  if (t >= a.total) return;
+  const MmProduct& p = a.p;
+  const int split = t / a.gx, n0 = (t - split * a.gx) * COLS;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = n0 + (lane & (LPR - 1)) * EPC, kl = lane / LPR;
+  const int k_begin = split * a.k_per_split, k_end = min(p.K, k_begin + a.k_per_split);   // multiples of 8
+  const E* w = reinterpret_cast<const E*>(p.b) + n;
+  const E* x = reinterpret_cast<const E*>(p.a);
+  float acc[MR][EPC];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) acc[m][e] = 0.f;
+  for (int k0 = k_begin + (wave * KL + kl) * 8; k0 < k_end; k0 += kRowWaves * KL * 8) {
+    if (n >= p.N) break;
+    uintx4 wv[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) wv[u] = *reinterpret_cast<const uintx4*>(w + (long long)(k0 + u) * p.ldb);
+    uintx4 xv[MR][8 / EPC];   // packed: eight rows of fp32 would not fit the registers
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+      for (int h = 0; h < 8 / EPC; ++h) xv[m][h] = reinterpret_cast<const uintx4*>(x + (long long)min(m, p.M - 1) * p.lda + k0)[h];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      float f[EPC];
+      row_unpack<KIND>(wv[u], f);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        float g[EPC];
+        row_unpack<KIND>(xv[m][u / EPC], g);
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) acc[m][e] = fmaf(g[u % EPC], f[e], acc[m][e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) {
+      float v = acc[m][e];
+#pragma unroll
+      for (int off = LPR; off < 64; off <<= 1) v += __shfl_xor(v, off);
+      acc[m][e] = v;
+    }
+  if (kl == 0) {
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+      for (int e = 0; e < EPC; e += 4)
+        *reinterpret_cast<floatx4*>(part + (wave * MR + m) * COLS + lane * EPC + e) = floatx4{acc[m][e], acc[m][e + 1], acc[m][e + 2], acc[m][e + 3]};
+  }
+  row_finish<KIND, MR>(a, part, COLS, n0, split);
+}
+// W [N,K] (rows of k): a wave owns one column of C at a time and its lanes go along k; 16 columns a workgroup and a
+// copy of x in LDS. The waves' sums need no joining.
+template <MmKind KIND, int MR>
+__global__ __launch_bounds__(64 * kRowWaves) void linear_row_k_kernel(LinTileArgs a) {
+  DTF_ABORT_GUARD(a);
+  using E = typename MmElem<KIND>::type;
+  constexpr int EPC = 16 / sizeof(E), DEEP = 4;
+  extern __shared__ __attribute__((aligned(16))) char lin_smem[];
+  const int t = mm_item(blockIdx.x, a.total);
+  if (t >= a.total) return;
+  const MmProduct& p = a.p;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int chunks = p.K / EPC;   // whole: K is a multiple of 8
+  uintx4* xs = reinterpret_cast<uintx4*>(lin_smem);   // [MR][chunks]
+  float* part = reinterpret_cast<float*>(lin_smem + (size_t)MR * chunks * 16);   // [MR][16]
+  const int n = t * kRowWaves + wave;
+  const uintx4* w = reinterpret_cast<const uintx4*>(reinterpret_cast<const E*>(p.b) + (long long)min(n, p.N - 1) * p.ldb);
+  uintx4 wv[DEEP];
+#pragma unroll
+  for (int u = 0; u < DEEP; ++u) wv[u] = lane + 64 * u < chunks ? w[lane + 64 * u] : uintx4{0, 0, 0, 0};
+  for (int e = threadIdx.x; e < MR * chunks; e += 64 * kRowWaves) {
+    const int m = e / chunks;
+    xs[e] = reinterpret_cast<const uintx4*>(reinterpret_cast<const E*>(p.a) + (long long)min(m, p.M - 1) * p.lda)[e - m * chunks];
+  }
+  __syncthreads();
+  float acc[MR];
+#pragma unroll
+  for (int m = 0; m < MR; ++m) acc[m] = 0.f;
+  for (int c0 = lane; c0 < chunks; c0 += 64 * DEEP) {
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) {
+      const int c = c0 + 64 * u;
+      if (c < chunks) {
+        float f[EPC];
+        row_unpack<KIND>(wv[u], f);
+        if (c + 64 * DEEP < chunks) wv[u] = w[c + 64 * DEEP];
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+          float g[EPC];
+          row_unpack<KIND>(xs[m * chunks + c], g);
+#pragma unroll
+          for (int e = 0; e < EPC; ++e) acc[m] = fmaf(g[e], f[e], acc[m]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MR; ++m) {
+    const float v = wave_sum(acc[m]);
+    if (lane == 0) part[m * kRowWaves + wave] = v;
+  }
+  __syncthreads();
+  if (threadIdx.x < MR * 4) {
+    const int m = threadIdx.x >> 2, c = (threadIdx.x & 3) * 4;
+    if (m < p.M && t * kRowWaves + c < p.N) lin_finish<KIND>(p, a.vec, m, t * kRowWaves + c, *reinterpret_cast<const floatx4*>(part + m * kRowWaves + c));
   }
 }
 
@@ -183,7 +399,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinDzArgs a) {
       if (a.act != ACT_NONE) {
         const floatx4 z = lin_load4<KIND>(a.pre, (long long)m * a.ldp + n, a.vec, have);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] *= lin_act_grad(a.act, z[i]);
+        for (int i = 0; i < 4; ++i) v[i] *= lin_act_grad<KIND>(a.act, z[i]);
       }
       if (a.dz) lin_store4<KIND>(a.dz, (long long)m * a.lddz + n, a.vec, have, v);
       s += v;
@@ -227,7 +443,7 @@ const LinLaunch& lin_launch_bf16();
 const LinLaunch& lin_launch_f16();
 
 // The variants of the product kernel: tile, waves over it, stages in LDS, 128-byte pieces of k per stage.
-enum LinVariant { LIN_REGS = 0, LIN_64 = 1, LIN_128 = 2, LIN_256 = 3 };
+enum LinVariant { LIN_REGS = 0, LIN_64 = 1, LIN_128 = 2, LIN_256 = 3, LIN_ROWS = 4 };
 struct LinTile { int t, wgm, wgn, stages, subs; };
 constexpr LinTile kLinTiles[] = {{128, 2, 2, 1, 1}, {64, 2, 2, 4, 1}, {128, 2, 4, 2, 2}, {256, 2, 4, 2, 1}};
 
@@ -248,6 +464,34 @@ void lin_tile_launch_as(const LinTileArgs& a, hipStream_t stream) {
   launch("linear", linear_tile_kernel<KIND, Loop, T.t, T.t, T.wgm, T.wgn>, dim3((unsigned)((a.total + 7) / 8 * 8)), dim3(64 * WAVES), lin_lds<Loop, WAVES>(),
          stream, a);
 }
+// columns of a workgroup of the few-rows kernel over W [K,N], by lanes side by side
+inline int lin_row_lanes(int N, int elems) {
+  const int groups = ceil_div(N, elems);   // chunks of columns
+  return groups >= 8 * 256 ? 8 : groups >= 4 * 256 ? 4 : 2;
+}
+template <MmKind KIND, int MR, bool KCB>
+void lin_row_launch_as(const LinTileArgs& a, hipStream_t stream) {
+  constexpr int EPC = MmTraits<KIND>::EPC;
+  const dim3 grid((unsigned)((a.total + 7) / 8 * 8)), block(64 * kRowWaves);
+  if (KCB) {
+    launch("linear_rows", linear_row_k_kernel<KIND, MR>, grid, block, (size_t)MR * a.p.K * (16 / EPC) + MR * kRowWaves * 4, stream, a);
+    return;
+  }
+  auto lds = [](int lanes) { return (size_t)kRowWaves * MR * lanes * EPC * 4; };
+  switch (lin_row_lanes(a.p.N, EPC)) {
+    case 2: launch("linear_rows", linear_row_n_kernel<KIND, MR, 2>, grid, block, lds(2), stream, a); break;
+    case 4: launch("linear_rows", linear_row_n_kernel<KIND, MR, 4>, grid, block, lds(4), stream, a); break;
+    default: launch("linear_rows", linear_row_n_kernel<KIND, MR, 8>, grid, block, lds(8), stream, a);
+  }
+}
+template <MmKind KIND, bool KCB>
+void lin_row_launch(const LinTileArgs& a, hipStream_t stream) {
+  if (a.p.M <= 1) lin_row_launch_as<KIND, 1, KCB>(a, stream);
+  else if (a.p.M <= 2) lin_row_launch_as<KIND, 2, KCB>(a, stream);
+  else if (a.p.M <= 4) lin_row_launch_as<KIND, 4, KCB>(a, stream);
+  else if constexpr (KIND == MM_F32) lin_row_launch_as<KIND, 8, KCB>(a, stream);
+  else throw std::runtime_error("linear: too many rows");
+}
 template <MmKind KIND, bool KCA, bool KCB>
 void lin_tile_launch(const LinTileArgs& a, int variant, hipStream_t stream) {
   switch (variant) {
@@ -255,6 +499,9 @@ void lin_tile_launch(const LinTileArgs& a, int variant, hipStream_t stream) {
     case LIN_64: return lin_tile_launch_as<KIND, KCA, KCB, LIN_64>(a, stream);
     case LIN_128: return lin_tile_launch_as<KIND, KCA, KCB, LIN_128>(a, stream);
     case LIN_256: return lin_tile_launch_as<KIND, KCA, KCB, LIN_256>(a, stream);
+    case LIN_ROWS:
+      if constexpr (KCA) return lin_row_launch<KIND, KCB>(a, stream);
+      [[fallthrough]];
     default: throw std::runtime_error("linear: unknown variant");
   }
 }

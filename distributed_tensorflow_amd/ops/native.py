@@ -1341,13 +1341,15 @@ def muon_step(p, g, m, v, hyper, tables: MuonTables, *, nesterov: bool, steps: i
 
 def linear_workspace(m: int, n: int, k: int, dtype=torch.float32, trans_w: bool = False) -> int:
     """Bytes of workspace that linear() may need for x [m,k] and n outputs, whatever the tensors' strides."""
-    return hip().linear_workspace(_KINDS[dtype], m, n, k, int(trans_w), 0, 0, k, 0, k if trans_w else n, 0, 0, 0, 0, n, 0, 0)
+    ldw = k if trans_w else n
+    return max(hip().linear_workspace(_KINDS[dtype], m, n, k, trans_w, 0, at, k, at, ldw, 0, 0, 0, 0, n, 0, 0) for at in (0, 1))   # aligned or not
 
 
 def linear_bwd_workspace(m: int, n: int, k: int, dtype=torch.float32, trans_w: bool = False, activation: str = "none") -> int:
     """Bytes of workspace that linear_bwd() may need for dy [m,n] and x [m,k] with all three gradients."""
     ldw = k if trans_w else n
-    return hip().linear_bwd_workspace(_KINDS[dtype], m, n, k, int(trans_w), ACTIVATIONS[activation], 0, 0, n, 0, n, 0, k, 0, ldw, 1, k, 1, ldw, 1)
+    return max(hip().linear_bwd_workspace(_KINDS[dtype], m, n, k, trans_w, ACTIVATIONS[activation], False, at, n, 0, n, at, k, at, ldw, 1, k, 1, ldw, 1)
+               for at in (0, 1))
 
 
 def col_sum(x2d, out, relu_of=None, masked=None):
