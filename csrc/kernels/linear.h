@@ -13,6 +13,7 @@ struct MmProduct {
   int M, N, K;
   const void* a; long long lda;
   const void* b; long long ldb;
+  int pad_a, pad_b;         // the operand's lines end in zeros up to a multiple of 16 bytes
   void* c; long long ldc;
   const void* bias;         // nullable, [N]
   const void* res;          // nullable, [M,N]: added after the activation

@@ -29,15 +29,26 @@ size_t round_up(size_t v) { return (v + 255) & ~(size_t)255; }
 struct Plan {
   int variant, splits, k_per_split, gx, gy;
   long long N4;
-  size_t bytes;
+  int copy_a, copy_b;            // the operand goes through a padded copy
+  long long ld_a, ld_b;          // leading dimension of the copy
+  size_t bytes, bytes_a, bytes_b;   // partial sums, copies
 };
 Plan plan_of(const MmProduct& p) {
   Plan l{};
-  const int es = elem_bytes(p.kind);
-  auto direct = [&](const void* base, long long ld, int contiguous) {
-    return aligned_to(base, 16) && !(ld * es & 15) && !((long long)contiguous * es & 15) && ld * es < (1 << 23);
+  const int es = elem_bytes(p.kind), epc = 16 / es;
+  // An operand can be loaded 16 bytes at a time if its lines start and end on multiples of them
+  auto direct = [&](const void* base, long long ld, int contiguous, int padded) {
+    return aligned_to(base, 16) && !(ld * es & 15) && (padded || !((long long)contiguous * es & 15)) && ld * es < (1 << 23);
   };
-  const bool whole = direct(p.a, p.lda, p.kc_a ? p.K : p.M) && direct(p.b, p.ldb, p.kc_b ? p.K : p.N);
+  const int line_a = p.kc_a ? p.K : p.M, line_b = p.kc_b ? p.K : p.N;
+  const bool ok_a = direct(p.a, p.lda, line_a, p.pad_a), ok_b = direct(p.b, p.ldb, line_b, p.pad_b);
+  bool whole = ok_a && ok_b;
+  // One that is not is copied where the product reads it often enough (fp16 1003 x 1531 x 2050: 35 -> 22 us)
+  if (!whole && p.M >= 64 && p.N >= 64 && p.K >= 64 && line_a < (1 << 20) && line_b < (1 << 20)) {
+    if (!ok_a) { l.copy_a = 1; l.ld_a = (line_a + epc - 1) / epc * epc; l.bytes_a = round_up((size_t)l.ld_a * (p.kc_a ? p.M : p.K) * es); }
+    if (!ok_b) { l.copy_b = 1; l.ld_b = (line_b + epc - 1) / epc * epc; l.bytes_b = round_up((size_t)l.ld_b * (p.kc_b ? p.N : p.K) * es); }
+    whole = true;
+  }
   const long long tiles128 = (long long)ceil_div(p.M, 128) * ceil_div(p.N, 128), tiles256 = (long long)ceil_div(p.M, 256) * ceil_div(p.N, 256);
   // The larger the tile the less it loads per product, as long as there is about a tile per CU (bf16, 256 / 128 / 64, us: 8192 x 4096 x 4096
   // 224 / 298 / 383, 2048 cubed 39 / 23 / 28, 512 x 2048 x 2048 - / 17.1 / 14.5; fp32 2048 cubed 148 / 127 / 134).
@@ -91,12 +102,16 @@ int dz_rows(int M, int N) {
 
 }  // namespace
 
-size_t mm_product_workspace(const MmProduct& p) { return p.M > 0 && p.N > 0 ? plan_of(p).bytes : 0; }
+size_t mm_product_workspace(const MmProduct& p) {
+  if (p.M <= 0 || p.N <= 0) return 0;
+  const Plan l = plan_of(p);
+  return l.bytes + l.bytes_a + l.bytes_b;
+}
 
 void mm_product(const MmProduct& p, void* ws, size_t ws_bytes, hipStream_t stream) {
   if (p.M <= 0 || p.N <= 0) return;
   const Plan l = plan_of(p);
-  check_ws("linear", l.bytes, ws, ws_bytes);
+  check_ws("linear", l.bytes + l.bytes_a + l.bytes_b, ws, ws_bytes);
   if ((long long)l.gx * l.gy * l.splits > 0x3fffffff) throw std::runtime_error("linear: the product has too many tiles");
   LinTileArgs a{};
   a.p = p;
@@ -104,7 +119,25 @@ void mm_product(const MmProduct& p, void* ws, size_t ws_bytes, hipStream_t strea
   a.N4 = l.N4;
   a.k_per_split = l.k_per_split;
   a.gx = l.gx; a.gy = l.gy; a.splits = l.splits; a.total = l.gx * l.gy * l.splits;
-  const int v4 = 4 * elem_bytes(p.kind);
+  const int es = elem_bytes(p.kind), epc = 16 / es, v4 = 4 * es;
+  auto up = [&](int n) { return (n + epc - 1) / epc * epc; };
+  if (l.copy_a || l.copy_b) {
+    LinPadArgs c{};
+    char* at = reinterpret_cast<char*>(ws) + l.bytes;
+    if (l.copy_a) {
+      c.src[0] = p.a; c.ld[0] = p.lda; c.dst[0] = at; c.ld_dst[0] = l.ld_a;
+      c.rows[0] = p.kc_a ? p.M : p.K; c.cols[0] = p.kc_a ? p.K : p.M;
+      a.p.a = at; a.p.lda = l.ld_a; a.p.pad_a = 1;
+    }
+    if (l.copy_b) {
+      c.src[1] = p.b; c.ld[1] = p.ldb; c.dst[1] = at + l.bytes_a; c.ld_dst[1] = l.ld_b;
+      c.rows[1] = p.kc_b ? p.N : p.K; c.cols[1] = p.kc_b ? p.K : p.N;
+      a.p.b = at + l.bytes_a; a.p.ldb = l.ld_b; a.p.pad_b = 1;
+    }
+    lin_launch(p.kind).pad(c, stream);
+  }
+  a.rows_a = !p.kc_a && a.p.pad_a ? up(p.M) : p.M;
+  a.rows_b = !p.kc_b && a.p.pad_b ? up(p.N) : p.N;
   a.vec = !(p.N & 3) && !(p.ldc & 3) && aligned_to(p.c, v4) && (!p.bias || aligned_to(p.bias, v4)) &&
           (!p.res || (!(p.ldr & 3) && aligned_to(p.res, v4))) && (!p.pre || (!(p.ldp & 3) && aligned_to(p.pre, v4)));
   const LinLaunch& f = lin_launch(p.kind);
@@ -146,6 +179,8 @@ BwdPlan bwd_plan(const LinearBwdArgs& a, void* dz) {
   b.dx.kind = a.kind;
   b.dx.kc_a = 1; b.dx.kc_b = !a.trans_w;
   b.dx.M = a.M; b.dx.N = a.K; b.dx.K = a.N;
+  b.dx.pad_a = own_dz;
+  (a.trans_w ? b.dw.pad_a : b.dw.pad_b) = own_dz;
   b.dx.a = src; b.dx.lda = ld; b.dx.b = a.w; b.dx.ldb = a.ldw;
   b.dx.c = a.dx; b.dx.ldc = a.lddx;
   // dw[K,N] = x^T dz, or [N,K] = dz^T x

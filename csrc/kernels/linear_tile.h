@@ -11,6 +11,7 @@ struct LinTileArgs {
   long long N4;
   int k_per_split;
   int gx, gy, total;   // tiles of C, and tiles x splits
+  int rows_a, rows_b;  // M and N for the loads: padded where the operand's contiguous dimension is
   int vec;             // four consecutive n can be read and written at once in every [M,N] tensor
   int splits;
   AbortRef abort;
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tile_kernel(LinTileArgs
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const MmOperands o{reinterpret_cast<const char*>(p.a), reinterpret_cast<const char*>(p.b), p.lda, p.ldb, p.M, p.N};
+  const MmOperands o{reinterpret_cast<const char*>(p.a), reinterpret_cast<const char*>(p.b), p.lda, p.ldb, a.rows_a, a.rows_b};
   Loop::run(o, m0, n0, k_begin, k_end, lin_smem, acc);
 
   // The sums leave through LDS, 32 rows of a wave's tile at a time: a loop over whole rows with 16 lanes to a row, so the
@@ -399,17 +400,54 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinDzArgs a) {
       if (a.act != ACT_NONE) {
         const floatx4 z = lin_load4<KIND>(a.pre, (long long)m * a.ldp + n, a.vec, have);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] *= lin_act_grad<KIND>(a.act, z[i]);
+        for (int i = 0; i < 4; ++i)
+          if (i < have) v[i] *= lin_act_grad<KIND>(a.act, z[i]);
       }
-      if (a.dz) lin_store4<KIND>(a.dz, (long long)m * a.lddz + n, a.vec, have, v);
+      if (a.dz) lin_store4<KIND>(a.dz, (long long)m * a.lddz + n, 1, 4, v);   // zeros past N
       s += v;
     }
+  } else if (a.dz && n < a.lddz) {
+    for (int m = m_begin + wave; m < m_end; m += 4) lin_store4<KIND>(a.dz, (long long)m * a.lddz + n, 1, 4, s);
   }
   if (!a.part) return;
   sums[wave][lane] = s;
   __syncthreads();
   if (wave == 0 && have > 0)
     *reinterpret_cast<floatx4*>(a.part + (long long)blockIdx.y * a.N4 + n) = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+}
+// Copies of operands that are not 16-byte aligned, lines padded with zeros: one pass over a matrix that a product reads many times.
+struct LinPadArgs {
+  const void* src[2]; void* dst[2];
+  long long ld[2], ld_dst[2];   // elements; ld_dst a multiple of 16 bytes
+  int rows[2], cols[2];
+  AbortRef abort;
+};
+template <MmKind KIND>
+__global__ __launch_bounds__(256) void linear_pad_kernel(LinPadArgs a) {
+  DTF_ABORT_GUARD(a);
+  using Raw = std::conditional_t<KIND == MM_F32, unsigned, unsigned short>;
+  constexpr int EPC = MmTraits<KIND>::EPC;
+  typedef Raw Chunk __attribute__((ext_vector_type(EPC)));
+  typedef Chunk __attribute__((aligned(2))) loose;
+  const int z = blockIdx.y;
+  const Raw* src = reinterpret_cast<const Raw*>(a.src[z]);
+  if (!src) return;
+  const int per_row = (int)(a.ld_dst[z] / EPC);
+  const long long count = (long long)per_row * a.rows[z], stride = (long long)gridDim.x * 256;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += stride) {
+    const long long row = i / per_row;
+    const int col = (int)(i - row * per_row) * EPC, have = a.cols[z] - col;
+    const Raw* p = src + row * a.ld[z] + col;
+    Chunk v = 0;
+    if (have >= EPC) {
+      v = *reinterpret_cast<const loose*>(p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPC; ++e)
+        if (e < have) v[e] = p[e];
+    }
+    *reinterpret_cast<Chunk*>(reinterpret_cast<Raw*>(a.dst[z]) + row * a.ld_dst[z] + col) = v;
+  }
 }
 struct LinColSumArgs { const float* part; long long N4; int blocks, N, accumulate; void* db; AbortRef abort; };
 template <MmKind KIND>
@@ -437,6 +475,7 @@ struct LinLaunch {
   void (*join)(const LinTileArgs&, hipStream_t);
   void (*dz)(const LinDzArgs&, dim3 grid, hipStream_t);
   void (*colsum)(const LinColSumArgs&, hipStream_t);
+  void (*pad)(const LinPadArgs&, hipStream_t);
 };
 const LinLaunch& lin_launch_f32();
 const LinLaunch& lin_launch_bf16();
@@ -522,6 +561,7 @@ LinLaunch lin_make_launch() {
     launch("linear_join", linear_join_kernel<KIND>, dim3((unsigned)(blocks > 4096 ? 4096 : blocks)), dim3(256), 0, s, a);
   };
   l.dz = [](const LinDzArgs& a, dim3 grid, hipStream_t s) { launch("linear_dz", linear_dz_kernel<KIND>, grid, dim3(256), 0, s, a); };
+  l.pad = [](const LinPadArgs& a, hipStream_t s) { launch("linear_pad", linear_pad_kernel<KIND>, dim3(1024, 2), dim3(256), 0, s, a); };
   l.colsum = [](const LinColSumArgs& a, hipStream_t s) {
     launch("linear_colsum", linear_colsum_kernel<KIND>, dim3((unsigned)ceil_div(a.N, 256)), dim3(256), 0, s, a);
   };
