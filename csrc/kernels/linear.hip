@@ -33,6 +33,25 @@ struct Plan {
   long long ld_a, ld_b;          // leading dimension of the copy
   size_t bytes, bytes_a, bytes_b;   // partial sums, copies
 };
+// The larger the tile the less is loaded per product, but it takes about a tile per CU to use the card. The choice goes by an
+// estimate: rounds of workgroups times stages of k, with the us of a round's stage measured with half the CUs busy and with all
+// (whole products, us by 64 / 128 / 256: bf16 8192 x 4096 x 4096 383 / 298 / 216, 2048 cubed 28 / 22 / 39, 1024 x 1536 x 2048 12.6 / 14.7 / -;
+// fp32 2048 cubed 132 / 125 / 148).
+struct TileCost { int variant, slots; float some16, full16, some32, full32; };
+constexpr TileCost kTileCosts[] = {{LIN_64, 512, 0.22f, 0.39f, 0.6f, 1.0f}, {LIN_128, 256, 0.55f, 0.6f, 1.8f, 1.92f}, {LIN_256, 256, 1.5f, 1.63f, 7.0f, 7.2f}};
+int pick_tile(const MmProduct& p) {
+  int best = LIN_64;
+  float least = 0.f;
+  for (const TileCost& c : kTileCosts) {
+    const int t = kLinTiles[c.variant].t;
+    const float n = (float)((long long)ceil_div(p.M, t) * ceil_div(p.N, t)) / (float)c.slots;
+    // two workgroups share a CU with 64 x 64 tiles: a round need not be full; else every round begun takes its time
+    const float rounds = n <= 1.f ? 1.f : c.slots > 256 ? n + 0.25f : ceilf(n);
+    const float us = rounds * (n <= 0.6f ? (p.kind == MM_F32 ? c.some32 : c.some16) : (p.kind == MM_F32 ? c.full32 : c.full16));
+    if (c.variant == LIN_64 || us < least) { best = c.variant; least = us; }
+  }
+  return best;
+}
 Plan plan_of(const MmProduct& p) {
   Plan l{};
   const int es = elem_bytes(p.kind), epc = 16 / es;
@@ -49,10 +68,7 @@ Plan plan_of(const MmProduct& p) {
     if (!ok_b) { l.copy_b = 1; l.ld_b = (line_b + epc - 1) / epc * epc; l.bytes_b = round_up((size_t)l.ld_b * (p.kc_b ? p.N : p.K) * es); }
     whole = true;
   }
-  const long long tiles128 = (long long)ceil_div(p.M, 128) * ceil_div(p.N, 128), tiles256 = (long long)ceil_div(p.M, 256) * ceil_div(p.N, 256);
-  // The larger the tile the less it loads per product, as long as there is about a tile per CU (bf16, 256 / 128 / 64, us: 8192 x 4096 x 4096
-  // 224 / 298 / 383, 2048 cubed 39 / 23 / 28, 512 x 2048 x 2048 - / 17.1 / 14.5; fp32 2048 cubed 148 / 127 / 134).
-  l.variant = !whole ? LIN_REGS : tiles256 >= 192 ? LIN_256 : tiles128 >= 128 ? LIN_128 : LIN_64;
+  l.variant = whole ? pick_tile(p) : LIN_REGS;
   const int kb = 128 / es;
   // A few rows: no tile is worth filling. x has to fit LDS where W's rows are along k.
   if (whole && p.kc_a && p.M <= lin_rows_max(p.kind) && !(p.K & 7) && p.K > 0 && (!p.kc_b || (long long)8 * p.K * es <= 128 * 1024)) {

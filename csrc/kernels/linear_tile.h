@@ -71,7 +71,8 @@ __device__ __forceinline__ float lin_act_grad(int act, float z) {
   }
 }
 
-// Four consecutive values of a tensor <-> fp32. `vec`: the address allows one access; else `have` of them, one by one.
+// Four consecutive values of a tensor <-> fp32. `vec`: they are there and aligned. Otherwise `have` of them are there, four in one
+// unaligned access, fewer one by one.
 template <MmKind KIND>
 __device__ __forceinline__ floatx4 lin_load4(const void* base, long long at, int vec, int have) {
   using E = typename MmElem<KIND>::type;
@@ -80,6 +81,9 @@ __device__ __forceinline__ floatx4 lin_load4(const void* base, long long at, int
   floatx4 v = {0.f, 0.f, 0.f, 0.f};
   if (vec) {
     v = __builtin_convertvector(*reinterpret_cast<const E4*>(p), floatx4);
+  } else if (have >= 4) {
+    typedef E4 __attribute__((aligned(2))) loose;
+    v = __builtin_convertvector(*reinterpret_cast<const loose*>(p), floatx4);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -94,6 +98,9 @@ __device__ __forceinline__ void lin_store4(void* base, long long at, int vec, in
   E* p = reinterpret_cast<E*>(base) + at;
   if (vec) {
     *reinterpret_cast<E4*>(p) = __builtin_convertvector(v, E4);
+  } else if (have >= 4) {
+    typedef E4 __attribute__((aligned(2))) loose;
+    *reinterpret_cast<loose*>(p) = __builtin_convertvector(v, E4);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -429,24 +436,25 @@ __global__ __launch_bounds__(256) void linear_pad_kernel(LinPadArgs a) {
   constexpr int EPC = MmTraits<KIND>::EPC;
   typedef Raw Chunk __attribute__((ext_vector_type(EPC)));
   typedef Chunk __attribute__((aligned(2))) loose;
-  const int z = blockIdx.y;
+  const int z = blockIdx.y, lane = threadIdx.x & 63;
   const Raw* src = reinterpret_cast<const Raw*>(a.src[z]);
   if (!src) return;
   const int per_row = (int)(a.ld_dst[z] / EPC);
-  const long long count = (long long)per_row * a.rows[z], stride = (long long)gridDim.x * 256;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += stride) {
-    const long long row = i / per_row;
-    const int col = (int)(i - row * per_row) * EPC, have = a.cols[z] - col;
-    const Raw* p = src + row * a.ld[z] + col;
-    Chunk v = 0;
-    if (have >= EPC) {
-      v = *reinterpret_cast<const loose*>(p);
-    } else {
+  for (int row = blockIdx.x * 4 + (threadIdx.x >> 6); row < a.rows[z]; row += gridDim.x * 4) {
+    const Raw* s = src + row * a.ld[z];
+    Chunk* d = reinterpret_cast<Chunk*>(reinterpret_cast<Raw*>(a.dst[z]) + row * a.ld_dst[z]);
+    for (int c = lane; c < per_row; c += 64) {
+      const int have = a.cols[z] - c * EPC;
+      Chunk v = 0;
+      if (have >= EPC) {
+        v = *reinterpret_cast<const loose*>(s + c * EPC);
+      } else {
 #pragma unroll
-      for (int e = 0; e < EPC; ++e)
-        if (e < have) v[e] = p[e];
+        for (int e = 0; e < EPC; ++e)
+          if (e < have) v[e] = s[c * EPC + e];
+      }
+      d[c] = v;
     }
-    *reinterpret_cast<Chunk*>(reinterpret_cast<Raw*>(a.dst[z]) + row * a.ld_dst[z] + col) = v;
   }
 }
 struct LinColSumArgs { const float* part; long long N4; int blocks, N, accumulate; void* db; AbortRef abort; };

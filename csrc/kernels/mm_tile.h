@@ -319,6 +319,7 @@ struct MmDirect {
       if (k_load < k_end) load();
     unsigned slot = 0;
     constexpr int GROUPS = MmTraits<KIND>::KS * MI, PIECES = OpA::NV + OpB::NV;
+    constexpr int RATE = (PIECES + GROUPS - 1) / GROUPS;
     int k0 = k_begin;
     // This stage has landed once no more than the loads issued after it are pending; near the end there are fewer.
     auto enter = [&]() {
@@ -335,7 +336,7 @@ struct MmDirect {
         const unsigned at = lds + slot_load + u * SUB;
         mm_stage<KIND, OpA, OpB, MI, NJ, SWAP>(As, As + OpA::BYTES, wm, wn, q, l15, acc, [&](int g) {
 #pragma unroll
-          for (int p = g * PIECES / GROUPS; p < (g + 1) * PIECES / GROUPS; ++p) {
+          for (int p = g * RATE; p < (g + 1) * RATE && p < PIECES; ++p) {
             if (p < OpA::NV) OpA::load_piece(p, pa, oa, at, wave);
             else OpB::load_piece(p - OpA::NV, pb, ob, at + OpA::BYTES, wave);
           }
