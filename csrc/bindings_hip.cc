@@ -551,7 +551,7 @@ PYBIND11_MODULE(_hip, m) {
     m.def("ns_shape", [](int rows, int cols) {
       NsMat x{};
       ns_shape(x, rows, cols);
-      return py::make_tuple(x.r, x.c, x.rp, x.cp, x.tall, x.parts, x.chunk, x.sx, ns_floats(x));
+      return py::make_tuple(x.r, x.c, x.rp, x.cp, x.tall, x.parts, x.chunk, x.sx, ns_floats(x), ns_small(x));
     });
     m.attr("NS_MAT_BYTES") = (int)sizeof(NsMat);
     m.attr("MUON_TILE") = kMuonTile;
@@ -560,8 +560,8 @@ PYBIND11_MODULE(_hip, m) {
     m.def("muon_step", [coeffs](const py::dict& d, uint64_t stream) {
       MuonArgs a{};
       P(p, float); P(g, const float); P(m, float); P(v, float); P(hyper, const float); P(mats, const NsMat);
-      P(items_flat, const NsItem); P(items_split, const NsItem); P(items_sym, const NsItem); P(items_apply, const NsItem);
-      V(n_flat); V(n_split); V(n_sym); V(n_apply); V(nesterov); V(eps); V(growth);
+      P(items_flat, const NsItem); P(items_small, const NsItem); P(items_split, const NsItem); P(items_sym, const NsItem); P(items_apply, const NsItem);
+      V(n_flat); V(n_small); V(n_out); V(n_split); V(n_sym); V(n_apply); V(nesterov); V(eps); V(growth);
       coeffs(d["coeffs"].cast<std::vector<float>>(), a.coeffs, a.steps);
       muon_step(a, as_ptr<void>(d, "ws"), as_stream(stream));
     });

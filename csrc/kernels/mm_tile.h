@@ -53,6 +53,12 @@ __device__ __forceinline__ void mm_mfma(int step, const Frag& x, const Frag& y, 
   }
 }
 
+template <MmKind KIND>
+__device__ __forceinline__ void mm_mfma_all(const Frag& x, const Frag& y, floatx4& acc) {
+#pragma unroll
+  for (int s = 0; s < MmSteps<KIND>::N; ++s) mm_mfma<KIND>(s, x, y, acc);
+}
+
 // 16 bytes per lane from memory to LDS at lds + 16 lane, past the registers; done when vmcnt says so. Written in asm
 // because the compiler, which cannot tell the two stages of a double buffer apart, would wait for every such load
 // before the next read of LDS. There is no output register.

@@ -38,6 +38,9 @@ __host__ __device__ inline long long ns_floats(const NsMat& m) { return 2 * kNsN
 // Fills in everything but the offsets.
 void ns_shape(NsMat& m, int rows, int cols);
 
+// Matrices whose steps all run in one workgroup.
+inline bool ns_small(const NsMat& m) { return m.r <= 32 ? m.c <= 1024 : m.r <= 64 && m.c <= 768; }
+
 struct NsItem { int mat, tile; };
 
 struct NsCoeffs { float a, b, c; };
@@ -63,7 +66,9 @@ struct MuonArgs {
   const float* hyper;
   const NsMat* mats;
   const NsItem* items_flat; int n_flat;     // (matrix, chunk of it), or (-1 - count, first element / kMuonVecAlign)
-  const NsItem* items_split; int n_split;
+  const NsItem* items_small; int n_small;   // matrices that ns_small covers, in none of the lists of tiles
+  const NsItem* items_split; int n_split;   // 32 x 32 blocks of every matrix, those of the small ones first:
+  int n_out;                                // this many
   const NsItem* items_sym; int n_sym;       // tiles of the r x r products, lower triangle
   const NsItem* items_apply; int n_apply;   // tiles of the r x c products
   int nesterov, steps;

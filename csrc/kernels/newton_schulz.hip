@@ -229,6 +229,21 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsDev a) {
   pair_store4(a.ws + ns_x(m), m.cp, bi * 32 + y, bj * 32 + x, floatx4{block[y][x], block[y][x + 1], block[y][x + 2], block[y][x + 3]});
 }
 
+// Element (row, col) of the output, or of the parameter that it updates.
+__device__ __forceinline__ void ns_write(const NsDev& a, const NsMat& m, int row, int col, float v, float lr, float decay) {
+  const long long at = m.out + (long long)row * m.out_ld + col;
+  if (a.m) {
+    float* p = reinterpret_cast<float*>(a.out) + at;
+    *p = decay * *p - lr * v;
+  } else if (a.kind == MM_F32) {
+    reinterpret_cast<float*>(a.out)[at] = v;
+  } else if (a.kind == MM_BF16) {
+    reinterpret_cast<__bf16*>(a.out)[at] = (__bf16)v;
+  } else {
+    reinterpret_cast<_Float16*>(a.out)[at] = (_Float16)v;
+  }
+}
+
 enum NsOp { NS_GRAM, NS_POLY, NS_APPLY };
 
 // Tiles: waves over T x T, stages in LDS, 128-byte pieces of k per stage; then what the choice between them goes by: workgroups
@@ -351,22 +366,254 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
       const int col = (m.tall ? m0 + wm + i * 16 : n0 + wn + j * 16) + 4 * q;
       if (row >= m.rows) continue;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (col + e >= m.cols) continue;
-        const long long at = m.out + (long long)row * m.out_ld + col + e;
-        const float v = acc[i][j][e] * f;
-        if (a.m) {
-          float* p = reinterpret_cast<float*>(a.out) + at;
-          *p = decay * *p - lr * v;
-        } else if (a.kind == MM_F32) {
-          reinterpret_cast<float*>(a.out)[at] = v;
-        } else if (a.kind == MM_BF16) {
-          reinterpret_cast<__bf16*>(a.out)[at] = (__bf16)v;
-        } else {
-          reinterpret_cast<_Float16*>(a.out)[at] = (_Float16)v;
+      for (int e = 0; e < 4; ++e)
+        if (col + e < m.cols) ns_write(a, m, row, col + e, acc[i][j][e] * f, lr, decay);
+    }
+}
+
+// ---- Small matrices: all steps in one workgroup of eight waves, X in registers.
+//
+// A wave owns up to four blocks of 32 columns of X, as the fragments that X X^T needs: lane (q, l15) has row 16 i + l15 and, of block b, the
+// columns 32 b + {4 q .. 4 q + 3, 16 + 4 q .. 16 + 4 q + 3} (any order of k serves a product whose operands share it, and this is the
+// order in which P X leaves the matrix pipe). A step: the waves' parts of X X^T are added in wave order in LDS, P is formed there, and
+// each wave turns its blocks round through LDS (transposed reads), multiplies them by P and has the next X. The kernel starts from
+// the pairs that ns_split_kernel wrote and leaves pairs for ns_out_kernel: reading and writing the matrices themselves here ran as slowly as
+// one CU can (35 us of a 6 x 576 x 64 call).
+constexpr int kSmallWaves = 8, kSmallPitch = 272, kTurnPitch = 144;   // bytes per row of A and P, and of a block being turned
+constexpr int kSmallPart = 10 * 1024;                                 // bytes of a wave's part of X X^T
+constexpr int kSmallLds = kSmallWaves * kSmallPart + 2 * 64 * kSmallPitch;
+static_assert(64 * kTurnPitch <= kSmallPart && kSmallLds <= (int)kLdsBudget, "LDS of the small-matrix kernel");
+
+// h and l of four values of row `row` of A or P, columns col .. col + 3
+__device__ __forceinline__ void small_store4(char* mat, int row, int col, const floatx4& v) {
+  halfx4 h, l;
+  pair_split(v, h, l);
+  char* p = mat + row * kSmallPitch + (col >> 5) * 128 + (col & 31) * 2;
+  *reinterpret_cast<halfx4*>(p) = h;
+  *reinterpret_cast<halfx4*>(p + 64) = l;
+}
+// four values of a symmetric matrix in both places
+__device__ __forceinline__ void small_store_sym(char* mat, int row, int col, const floatx4& v, bool mirror) {
+  small_store4(mat, row, col, v);
+  if (!mirror) return;
+  halfx4 h, l;
+  pair_split(v, h, l);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    _Float16* p = reinterpret_cast<_Float16*>(mat + (col + e) * kSmallPitch + (row >> 5) * 128) + (row & 31);
+    p[0] = h[e];
+    p[32] = l[e];
+  }
+}
+
+template <int RT, int NB>   // 16-row tiles of X, blocks of a wave (those past X's columns are zeros)
+__device__ __forceinline__ void ns_small_run(const NsDev& a, const NsMat& m, const NsCoeffs* co, int steps, char* smem) {
+  constexpr int KBS = (RT + 1) / 2, TILES = RT * (RT + 1) / 2;   // 32-row blocks of X, tiles on and below the diagonal
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, l15 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  char *parts = smem, *A = smem + kSmallWaves * kSmallPart, *P = A + 64 * kSmallPitch;
+  char* mine = parts + wave * kSmallPart;
+  for (int e = tid; e < 2 * 64 * kSmallPitch / 16; e += 64 * kSmallWaves) reinterpret_cast<uintx4*>(A)[e] = uintx4{0, 0, 0, 0};
+
+  float* X = a.ws + ns_x(m);
+  Frag F[RT][NB];
+#pragma unroll
+  for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int row = 16 * i + l15, col = 32 * (kb * kSmallWaves + wave);
+      uintx2 v[4] = {};
+      if (row < m.rp && col < m.cp) {
+        const char* p = reinterpret_cast<const char*>(X + (long long)row * m.cp + col) + q * 8;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const uintx2*>(p + 32 * u);   // h, h, l, l
+      }
+      F[i][kb].h = uintx4{v[0][0], v[0][1], v[1][0], v[1][1]};
+      F[i][kb].l = uintx4{v[2][0], v[2][1], v[3][0], v[3][1]};
+    }
+  float tau = a.ws[m.ws + 2 * kNsNormParts];
+  __syncthreads();
+
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    // the wave's part of X X^T: lane (q, l15) of a tile has row 16 i + l15, columns 16 j + 4 q ..
+    {
+      floatx4 acc[TILES];
+#pragma unroll
+      for (int k = 0; k < TILES; ++k) acc[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int s = 0; s < 3; ++s)
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j <= i; ++j) mm_mfma<MM_PAIR>(s, F[j][kb], F[i][kb], acc[i * (i + 1) / 2 + j]);
+#pragma unroll
+      for (int k = 0; k < TILES; ++k) *reinterpret_cast<floatx4*>(mine + k * 1024 + lane * 16) = acc[k];
+    }
+    __syncthreads();
+    for (int e = tid; e < TILES * 64; e += 64 * kSmallWaves) {
+      floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kSmallWaves; ++w) s += *reinterpret_cast<const floatx4*>(parts + w * kSmallPart + e * 16);
+      const int k = e >> 6, i = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, j = k - i * (i + 1) / 2;
+      small_store_sym(A, 16 * i + (e & 15), 16 * j + 4 * ((e >> 4) & 3), s * (kScaleA / (m.sx * m.sx)), i != j);
+    }
+    __syncthreads();
+    const float next = fminf(1.f, tau * a.growth);
+    {
+      const float s1 = kScaleP * (tau / next), t2 = tau * tau;
+      const float ca = s1 * co[step].a, cb = s1 * co[step].b * t2 * (1.f / kScaleA), cc = s1 * co[step].c * t2 * t2 * (1.f / (kScaleA * kScaleA));
+      for (int k = wave; k < TILES; k += kSmallWaves) {
+        const int i = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, j = k - i * (i + 1) / 2;
+        floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < KBS; ++kb) {
+          auto frag = [&](int tile) {
+            const char* p = A + (16 * tile + l15) * kSmallPitch + kb * 128 + q * 16;
+            Frag f;
+            f.h = *reinterpret_cast<const uintx4*>(p);
+            f.l = *reinterpret_cast<const uintx4*>(p + 64);
+            return f;
+          };
+          mm_mfma_all<MM_PAIR>(frag(j), frag(i), acc);
         }
+        const int row = 16 * i + l15, col = 16 * j + 4 * q;
+        const char* p = A + row * kSmallPitch + (col >> 5) * 128 + (col & 31) * 2;
+        floatx4 x = acc * cc + (__builtin_convertvector(*reinterpret_cast<const halfx4*>(p), floatx4) +
+                                __builtin_convertvector(*reinterpret_cast<const halfx4*>(p + 64), floatx4)) * cb;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (row == col + e && row < m.r) x[e] += ca;
+        small_store_sym(P, row, col, x, i != j);
       }
     }
+    // The blocks, rows as lines, into the wave's own memory (free since the barrier behind the sums) and back with columns as lanes.
+    Frag G[NB][KBS][2];
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        char* p = mine + (16 * i + l15) * kTurnPitch + q * 8;
+        *reinterpret_cast<uintx2*>(p) = uintx2{F[i][kb].h[0], F[i][kb].h[1]};
+        *reinterpret_cast<uintx2*>(p + 32) = uintx2{F[i][kb].h[2], F[i][kb].h[3]};
+        *reinterpret_cast<uintx2*>(p + 64) = uintx2{F[i][kb].l[0], F[i][kb].l[1]};
+        *reinterpret_cast<uintx2*>(p + 96) = uintx2{F[i][kb].l[2], F[i][kb].l[3]};
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");   // this wave's lines are there; the reads stay behind them
+#pragma unroll
+      for (int kk = 0; kk < KBS; ++kk)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const unsigned char* p = reinterpret_cast<const unsigned char*>(mine) + (32 * kk + 4 * q + (l15 >> 2)) * kTurnPitch + c * 32 + (l15 & 3) * 8;
+          const uintx2 h0 = lds_read_tr(p), l0 = lds_read_tr(p + 64);
+          uintx2 h1 = {0, 0}, l1 = {0, 0};
+          if (RT > 1) {
+            h1 = lds_read_tr(p + 16 * kTurnPitch);
+            l1 = lds_read_tr(p + 16 * kTurnPitch + 64);
+          }
+          G[kb][kk][c].h = uintx4{h0[0], h0[1], h1[0], h1[1]};
+          G[kb][kk][c].l = uintx4{l0[0], l0[1], l1[0], l1[1]};
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");   // read before the next block's lines are written
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      Frag w[KBS];
+#pragma unroll
+      for (int kk = 0; kk < KBS; ++kk) {
+        const char* p = P + (16 * i + l15) * kSmallPitch + kk * 128 + q * 8;
+        const uintx2 h0 = *reinterpret_cast<const uintx2*>(p), h1 = *reinterpret_cast<const uintx2*>(p + 32);
+        const uintx2 l0 = *reinterpret_cast<const uintx2*>(p + 64), l1 = *reinterpret_cast<const uintx2*>(p + 96);
+        w[kk].h = uintx4{h0[0], h0[1], h1[0], h1[1]};
+        w[kk].l = uintx4{l0[0], l0[1], l1[0], l1[1]};
+      }
+      floatx4 acc[NB][2];
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) acc[kb][0] = acc[kb][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KBS; ++kk)
+#pragma unroll
+        for (int s = 0; s < 3; ++s)
+#pragma unroll
+          for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) mm_mfma<MM_PAIR>(s, G[kb][kk][c], w[kk], acc[kb][c]);
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) {
+        halfx4 h[2], l[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) pair_split(acc[kb][c] * (1.f / kScaleP), h[c], l[c]);
+        F[i][kb].h = __builtin_bit_cast(uintx4, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        F[i][kb].l = __builtin_bit_cast(uintx4, __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    }
+    tau = next;
+    __syncthreads();   // the waves' memory, A and P are free
+  }
+#pragma unroll
+  for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int row = 16 * i + l15, col = 32 * (kb * kSmallWaves + wave);
+      if (row < m.rp && col < m.cp) {
+        char* p = reinterpret_cast<char*>(X + (long long)row * m.cp + col) + q * 8;
+        *reinterpret_cast<uintx2*>(p) = uintx2{F[i][kb].h[0], F[i][kb].h[1]};
+        *reinterpret_cast<uintx2*>(p + 32) = uintx2{F[i][kb].h[2], F[i][kb].h[3]};
+        *reinterpret_cast<uintx2*>(p + 64) = uintx2{F[i][kb].l[0], F[i][kb].l[1]};
+        *reinterpret_cast<uintx2*>(p + 96) = uintx2{F[i][kb].l[2], F[i][kb].l[3]};
+      }
+    }
+  if (tid == 0) a.ws[m.ws + 2 * kNsNormParts] = tau;
+}
+struct NsSmallArgs { NsDev d; int steps; NsCoeffs co[kNsMaxSteps]; };
+__global__ __launch_bounds__(64 * kSmallWaves) void ns_small_kernel(NsSmallArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char ns_smem[];
+  NsMat m;
+  int tile;
+  ns_find(a.d, blockIdx.x, m, tile);
+  const int nb = (m.c + 32 * kSmallWaves - 1) / (32 * kSmallWaves);
+#define NS_SMALL(RT, NB) ns_small_run<RT, NB>(a.d, m, a.co, a.steps, ns_smem)
+  if (m.r <= 16) {
+    if (nb == 1) NS_SMALL(1, 1);
+    else NS_SMALL(1, 4);
+  } else if (m.r <= 32) {
+    if (nb <= 2) NS_SMALL(2, 2);
+    else NS_SMALL(2, 4);
+  } else if (nb == 1) {
+    NS_SMALL(4, 1);
+  } else {
+    NS_SMALL(4, 3);
+  }
+#undef NS_SMALL
+}
+// What ns_small_kernel left, into the output or the parameter: one 32 x 32 block of X per workgroup.
+__global__ __launch_bounds__(256) void ns_out_kernel(NsDev a) {
+  __shared__ float block[32][33];
+  NsMat m;
+  int tile;
+  ns_find(a, blockIdx.x, m, tile);
+  const int bc = m.cp / 32, bi = tile / bc, bj = tile - bi * bc;
+  {
+    const int y = threadIdx.x >> 3, x = (threadIdx.x & 7) * 4;
+    const floatx4 v = pair_load4(a.ws + ns_x(m), m.cp, bi * 32 + y, bj * 32 + x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (m.tall) block[x + e][y] = v[e];
+      else block[y][x + e] = v[e];
+    }
+  }
+  __syncthreads();
+  const float f = a.ws[m.ws + 2 * kNsNormParts] / m.sx;
+  const float lr = a.m ? a.hyper[0] * m.scale : 0.f, decay = a.m ? a.hyper[3] : 0.f;
+  const int r0 = (m.tall ? bj : bi) * 32, c0 = (m.tall ? bi : bj) * 32;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int y = (threadIdx.x >> 5) + 8 * k, x = threadIdx.x & 31;
+    if (r0 + y < m.rows && c0 + x < m.cols) ns_write(a, m, r0 + y, c0 + x, block[y][x] * f, lr, decay);
+  }
 }
 
 template <NsOp OP>
@@ -440,6 +687,15 @@ void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t strea
   launch("ns_norm", ns_norm_kernel, dim3(n.total), dim3(256), 0, stream, n);
   const NsDev s = with((m.rp / 32) * (m.cp / 32));
   launch("ns_split", ns_split_kernel, dim3(s.total), dim3(256), 0, stream, s);
+  if (ns_small(m)) {
+    NsSmallArgs k{};
+    k.d = with(1);
+    k.steps = a.steps;
+    for (int i = 0; i < a.steps; ++i) k.co[i] = a.coeffs[i];
+    launch("ns_small", ns_small_kernel, dim3(k.d.total), dim3(64 * kSmallWaves), kSmallLds, stream, k);
+    launch("ns_out", ns_out_kernel, dim3(s.total), dim3(256), 0, stream, s);
+    return;
+  }
   const int tg = pick_tile([&](int T) { return (long long)sym_tiles(m, T) * a.batch; }, m.cp / 32);
   const int tp = pick_tile([&](int T) { return (long long)sym_tiles(m, T) * a.batch; }, m.rp / 32);
   const int ta = pick_tile([&](int T) { return (long long)apply_tiles(m, T) * a.batch; }, m.rp / 32);
@@ -469,6 +725,15 @@ void muon_step(const MuonArgs& a, void* ws, hipStream_t stream) {
   if (a.n_flat > 0) launch("muon_flat", muon_flat_kernel, dim3(a.n_flat), dim3(256), 0, stream, with(a.items_flat, a.n_flat));
   if (a.n_split <= 0) return;
   launch("muon_split", ns_split_kernel, dim3(a.n_split), dim3(256), 0, stream, with(a.items_split, a.n_split));
+  if (a.n_small > 0) {
+    NsSmallArgs s{};
+    s.d = with(a.items_small, a.n_small);
+    s.steps = a.steps;
+    for (int k = 0; k < a.steps; ++k) s.co[k] = a.coeffs[k];
+    launch("muon_small", ns_small_kernel, dim3(a.n_small), dim3(64 * kSmallWaves), kSmallLds, stream, s);
+    launch("muon_out", ns_out_kernel, dim3(a.n_out), dim3(256), 0, stream, with(a.items_split, a.n_out));
+  }
+  if (a.n_sym <= 0) return;
   for (int k = 0; k < a.steps; ++k) {
     d.step = k;
     d.last = k == a.steps - 1;

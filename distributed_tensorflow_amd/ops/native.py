@@ -1301,14 +1301,19 @@ class MuonTables:
         h = hip()
         assert self.MAT.itemsize == h.NS_MAT_BYTES
         mats = np.zeros(len(matrices), dtype=self.MAT)
-        flat, split, sym, apply, floats, tile = [], [], [], [], 0, h.MUON_TILE
+        flat, small, out, split, sym, apply, floats, tile = [], [], [], [], [], [], 0, h.MUON_TILE
         for i, (off, rows, cols) in enumerate(matrices):
-            r, c, rp, cp, tall, parts, chunk, sx, need = h.ns_shape(rows, cols)
+            r, c, rp, cp, tall, parts, chunk, sx, need, is_small = h.ns_shape(rows, cols)
             mats[i] = (off, off, cols, cols, floats, rows, cols, r, c, rp, cp, tall, parts, chunk, sx, math.sqrt(max(1.0, cols / rows)), 0)
             floats += (need + 63) // 64 * 64
             tr, tc = -(-rp // tile), -(-cp // tile)
             flat += [(i, k) for k in range(parts)]
-            split += [(i, k) for k in range((rp // 32) * (cp // 32))]
+            blocks = [(i, k) for k in range((rp // 32) * (cp // 32))]
+            if is_small:
+                small.append((i, 0))
+                out += blocks
+                continue
+            split += blocks
             sym += [(i, k) for k in range(tr * (tr + 1) // 2)]
             apply += [(i, k) for k in range(tr * tc)]
         for off, n in vectors:
@@ -1318,11 +1323,12 @@ class MuonTables:
                 flat.append((-1 - min(h.MUON_VEC_CHUNK, n - k), (off + k) // h.MUON_VEC_ALIGN))
         self.workspace = torch.empty(max(1, floats), device=device, dtype=torch.float32)
         self._mats = torch.from_numpy(mats.view(np.uint8).copy()).to(device)
-        self._items = [torch.tensor(x, dtype=torch.int32).reshape(-1, 2).to(device) for x in (flat, split, sym, apply)]
+        self._items = [torch.tensor(x, dtype=torch.int32).reshape(-1, 2).to(device) for x in (flat, small, out + split, sym, apply)]
+        self._out = len(out)
 
     def launch_args(self) -> dict:
-        d = dict(mats=self._mats.data_ptr(), ws=self.workspace.data_ptr())
-        for name, t in zip(("flat", "split", "sym", "apply"), self._items):
+        d = dict(mats=self._mats.data_ptr(), ws=self.workspace.data_ptr(), n_out=self._out)
+        for name, t in zip(("flat", "small", "split", "sym", "apply"), self._items):
             d["items_" + name], d["n_" + name] = t.data_ptr(), t.shape[0]
         return d
 
