@@ -553,6 +553,12 @@ PYBIND11_MODULE(_hip, m) {
       ns_shape(x, rows, cols);
       return py::make_tuple(x.r, x.c, x.rp, x.cp, x.tall, x.parts, x.chunk, x.sx, ns_floats(x), ns_small(x));
     });
+    m.def("ns_splits", [](int rows, int cols, long long tiles) {
+      NsMat x{};
+      ns_shape(x, rows, cols);
+      return ns_splits(x, tiles);
+    });
+    m.attr("NS_ITEM_BYTES") = (int)sizeof(NsItem);
     m.attr("NS_MAT_BYTES") = (int)sizeof(NsMat);
     m.attr("MUON_TILE") = kMuonTile;
     m.attr("MUON_VEC_CHUNK") = kMuonVecChunk;
@@ -560,8 +566,8 @@ PYBIND11_MODULE(_hip, m) {
     m.def("muon_step", [coeffs](const py::dict& d, uint64_t stream) {
       MuonArgs a{};
       P(p, float); P(g, const float); P(m, float); P(v, float); P(hyper, const float); P(mats, const NsMat);
-      P(items_flat, const NsItem); P(items_small, const NsItem); P(items_split, const NsItem); P(items_sym, const NsItem); P(items_apply, const NsItem);
-      V(n_flat); V(n_small); V(n_out); V(n_split); V(n_sym); V(n_apply); V(nesterov); V(eps); V(growth);
+      P(items_flat, const NsItem); P(items_small, const NsItem); P(items_split, const NsItem); P(items_gram, const NsItem); P(items_join, const NsItem); P(parts, float); P(items_sym, const NsItem); P(items_apply, const NsItem);
+      V(n_flat); V(n_small); V(n_out); V(n_split); V(n_gram); V(n_sym); V(n_apply); V(nesterov); V(eps); V(growth);
       coeffs(d["coeffs"].cast<std::vector<float>>(), a.coeffs, a.steps);
       muon_step(a, as_ptr<void>(d, "ws"), as_stream(stream));
     });

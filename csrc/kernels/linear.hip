@@ -88,13 +88,13 @@ Plan plan_of(const MmProduct& p) {
   l.gx = ceil_div(p.N, tile);
   l.gy = ceil_div(p.M, tile);
   l.N4 = ((long long)p.N + 3) / 4 * 4;
-  // Few tiles and a long k: several workgroups share a tile's k, at least eight stages each, until two stand on every CU
+  // Few tiles and a long k: several workgroups share a tile's k, twelve stages each at least, until two stand on every CU
   // (fp32 128 x 3136 x 512, 64 x 64 tiles, us in 1 / 4 / 8 / 16 parts: 40 / 22.4 / 19.0 / 18.8, the host's time).
   const long long tiles = (long long)l.gx * l.gy;
   const int stages = ceil_div(p.K, kb);
   const int slots = l.variant == LIN_REGS || l.variant == LIN_64 ? 512 : 256;
   int splits = 1;
-  while (tiles * splits * 2 <= slots && stages >= splits * 16 && (size_t)p.M * l.N4 * splits * 8 <= kMaxPartialBytes) splits *= 2;
+  while (tiles * splits * 2 <= slots && stages >= splits * 24 && (size_t)p.M * l.N4 * splits * 8 <= kMaxPartialBytes) splits *= 2;
   const int per = ceil_div(stages, splits) * kb;
   l.splits = p.K > 0 ? ceil_div(p.K, per) : 1;
   l.k_per_split = p.K > 0 ? per : kb;

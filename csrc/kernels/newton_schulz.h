@@ -41,7 +41,17 @@ void ns_shape(NsMat& m, int rows, int cols);
 // Matrices whose steps all run in one workgroup.
 inline bool ns_small(const NsMat& m) { return m.r <= 32 ? m.c <= 1024 : m.r <= 64 && m.c <= 768; }
 
-struct NsItem { int mat, tile; };
+// A work item. Split X X^T: kn blocks of 32 columns of X from k0 on, its sums into slot `slot`; joining it: kn slots from `slot` on.
+struct NsItem { int mat, tile, k0, kn, slot, pad; };
+constexpr int kNsSplitTile = 64;
+constexpr int kNsSplitMax = 8;
+// Parts that X X^T is computed in where `tiles` 64 x 64 tiles in all leave CUs idle: twelve blocks of k each at least.
+inline int ns_splits(const NsMat& m, long long tiles) {
+  long long s = tiles > 0 ? 512 / tiles : 1;
+  if (s > kNsSplitMax) s = kNsSplitMax;
+  if (s > m.cp / (12 * 32)) s = m.cp / (12 * 32);
+  return s < 1 ? 1 : (int)s;
+}
 
 struct NsCoeffs { float a, b, c; };
 
@@ -69,9 +79,12 @@ struct MuonArgs {
   const NsItem* items_small; int n_small;   // matrices that ns_small covers, in none of the lists of tiles
   const NsItem* items_split; int n_split;   // 32 x 32 blocks of every matrix, those of the small ones first:
   int n_out;                                // this many
+  const NsItem* items_gram; int n_gram;     // parts of the tiles of X X^T, and their joining (tiles as items_sym)
+  const NsItem* items_join;
   const NsItem* items_sym; int n_sym;       // tiles of the r x r products, lower triangle
   const NsItem* items_apply; int n_apply;   // tiles of the r x c products
   int nesterov, steps;
+  float* parts;                             // 4096 floats per item of items_gram
   double eps;
   NsCoeffs coeffs[kNsMaxSteps];
   float growth;

@@ -36,6 +36,8 @@ struct NsDev {
   int step, last;
   float growth;
   NsCoeffs co;
+  int splits;                  // parts of a tile of X X^T, table == nullptr
+  float* parts;                // their sums, as the accumulators lie in the registers of a workgroup
 };
 
 __device__ __forceinline__ void ns_find(const NsDev& a, int t, NsMat& m, int& tile) {
@@ -244,7 +246,7 @@ __device__ __forceinline__ void ns_write(const NsDev& a, const NsMat& m, int row
   }
 }
 
-enum NsOp { NS_GRAM, NS_POLY, NS_APPLY };
+enum NsOp { NS_GRAM, NS_POLY, NS_APPLY, NS_GRAM_PART, NS_GRAM_JOIN };
 
 // Tiles: waves over T x T, stages in LDS, 128-byte pieces of k per stage; then what the choice between them goes by: workgroups
 // that the card holds at a time, and us per 32 of k of one round of them with half the CUs busy and with all (measured on 576 x 64 to
@@ -267,8 +269,26 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
   const int t = mm_item(blockIdx.x, a.total);
   if (t >= a.total) return;
   NsMat m;
-  int tile;
-  ns_find(a, t, m, tile);
+  int tile, k0 = 0, kn = 0;
+  long long slot = 0;
+  if (OP == NS_GRAM_PART && !a.table) {   // the parts of one range of k together: they share rows of X in an XCD's L2
+    const int tiles = a.total / a.splits, part = t / tiles, i = t - part * tiles;
+    ns_find(a, i, m, tile);
+    const int all = m.cp >> 5;
+    k0 = all * part / a.splits;
+    kn = all * (part + 1) / a.splits - k0;
+    slot = (long long)i * a.splits + part;
+  } else {
+    ns_find(a, t, m, tile);
+    if (a.table) {
+      k0 = a.items[t].k0;
+      kn = a.items[t].kn;
+      slot = a.items[t].slot;
+    } else {
+      kn = a.splits;
+      slot = (long long)t * a.splits;
+    }
+  }
   int tx, ty;
   if (OP == NS_APPLY) {
     mm_tile_of(tile, (m.cp + T - 1) / T, (m.rp + T - 1) / T, tx, ty);
@@ -293,13 +313,31 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
   const int wm = (wave / WGN) * (T / WGM), wn = (wave % WGN) * (T / WGN);
 
   if (OP != NS_APPLY) {
-    const float* src = OP == NS_GRAM ? xa : A;
-    const int pitch = OP == NS_GRAM ? m.cp : m.rp;
-    const char* s = reinterpret_cast<const char*>(src);
-    NsLoop<T, true, true>::run(MmOperands{s, s, pitch, pitch, m.rp, m.rp}, m0, n0, 0, pitch, ns_smem, acc);
-    float* dst = OP == NS_GRAM ? A : P;
+    constexpr bool GRAM = OP != NS_POLY;
+    if constexpr (OP == NS_GRAM_JOIN) {
+      const floatx4* s = reinterpret_cast<const floatx4*>(a.parts) + slot * (MI * NJ * NsTile<T>::NT) + threadIdx.x;
+      for (int p = 0; p < kn; ++p)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j] += s[((p * MI + i) * NJ + j) * NsTile<T>::NT];
+    } else {
+      const int pitch = GRAM ? m.cp : m.rp;
+      const char* s = reinterpret_cast<const char*>(GRAM ? xa : A);
+      const int kb = OP == NS_GRAM_PART ? k0 * 32 : 0, ke = OP == NS_GRAM_PART ? (k0 + kn) * 32 : pitch;
+      NsLoop<T, true, true>::run(MmOperands{s, s, pitch, pitch, m.rp, m.rp}, m0, n0, kb, ke, ns_smem, acc);
+    }
+    if constexpr (OP == NS_GRAM_PART) {
+      floatx4* d = reinterpret_cast<floatx4*>(a.parts) + slot * (MI * NJ * NsTile<T>::NT) + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) d[(i * NJ + j) * NsTile<T>::NT] = acc[i][j];
+      return;
+    }
+    float* dst = GRAM ? A : P;
     float ca = 0.f, cb = 0.f, cc;   // value = ca I + cb A + cc acc
-    if (OP == NS_GRAM) {
+    if (GRAM) {
       cc = kScaleA / (m.sx * m.sx);
     } else {
       const float tau = tau_at(a.ws[m.ws + 2 * kNsNormParts], a.growth, a.step), next = fminf(1.f, tau * a.growth);
@@ -616,6 +654,12 @@ __global__ __launch_bounds__(256) void ns_out_kernel(NsDev a) {
   }
 }
 
+void gram_in_parts(const char* part, const char* join, const NsDev& p, const NsDev& j, hipStream_t stream) {
+  constexpr int T = kNsSplitTile;
+  const size_t lds = NsLoop<T, true, true>::LDS;
+  launch(part, ns_product_kernel<NS_GRAM_PART, T>, dim3((unsigned)((p.total + 7) / 8 * 8)), dim3(NsTile<T>::NT), lds, stream, p);
+  launch(join, ns_product_kernel<NS_GRAM_JOIN, T>, dim3((unsigned)((j.total + 7) / 8 * 8)), dim3(NsTile<T>::NT), 0, stream, j);
+}
 template <NsOp OP>
 void product(const char* name, NsDev d, int tile, hipStream_t stream) {
   const dim3 grid((unsigned)((d.total + 7) / 8 * 8));
@@ -658,10 +702,21 @@ void ns_shape(NsMat& m, int rows, int cols) {
   m.sx = s;
 }
 
+namespace {
+// parts of X X^T of a uniform call, 1 where a tile kernel does it alone
+int gram_splits(const NsMat& m, int batch) {
+  const long long tiles = (long long)sym_tiles(m, kNsSplitTile) * batch;
+  if (ns_small(m) || pick_tile([&](int T) { return (long long)sym_tiles(m, T) * batch; }, m.cp / 32) != kNsSplitTile) return 1;
+  return ns_splits(m, tiles);
+}
+}  // namespace
+
 size_t ns_workspace(const NsArgs& a) {
   NsMat m{};
   ns_shape(m, a.rows, a.cols);
-  return (size_t)ns_floats(m) * sizeof(float) * a.batch;
+  const int s = gram_splits(m, a.batch);
+  const long long parts = s > 1 ? (long long)sym_tiles(m, kNsSplitTile) * a.batch * s * kNsSplitTile * kNsSplitTile : 0;
+  return (size_t)(ns_floats(m) * a.batch + parts) * sizeof(float);
 }
 
 void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t stream) {
@@ -696,6 +751,10 @@ void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t strea
     launch("ns_out", ns_out_kernel, dim3(s.total), dim3(256), 0, stream, s);
     return;
   }
+  // X X^T of few rows and many columns: in parts, which are added in order (us of 512 x 3136 26 -> 13, of 1024 x 4096 36 -> 22)
+  const int splits = gram_splits(m, a.batch);
+  d.splits = splits;
+  d.parts = d.ws + ns_floats(m) * a.batch;
   const int tg = pick_tile([&](int T) { return (long long)sym_tiles(m, T) * a.batch; }, m.cp / 32);
   const int tp = pick_tile([&](int T) { return (long long)sym_tiles(m, T) * a.batch; }, m.rp / 32);
   const int ta = pick_tile([&](int T) { return (long long)apply_tiles(m, T) * a.batch; }, m.rp / 32);
@@ -703,7 +762,13 @@ void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t strea
     d.step = k;
     d.last = k == a.steps - 1;
     d.co = a.coeffs[k];
-    product<NS_GRAM>("ns_gram", with(sym_tiles(m, tg)), tg, stream);
+    if (splits > 1) {
+      NsDev p = with(sym_tiles(m, kNsSplitTile)), j = p;
+      p.total *= splits;
+      gram_in_parts("ns_gram_part", "ns_gram_join", p, j, stream);
+    } else {
+      product<NS_GRAM>("ns_gram", with(sym_tiles(m, tg)), tg, stream);
+    }
     product<NS_POLY>("ns_poly", with(sym_tiles(m, tp)), tp, stream);
     product<NS_APPLY>("ns_apply", with(apply_tiles(m, ta)), ta, stream);
   }
@@ -715,7 +780,7 @@ void muon_step(const MuonArgs& a, void* ws, hipStream_t stream) {
   d.table = a.mats;
   d.ws = reinterpret_cast<float*>(ws);
   d.g = a.g; d.out = a.p; d.m = a.m; d.v = a.v; d.hyper = a.hyper; d.kind = MM_F32;
-  d.nesterov = a.nesterov; d.eps = a.eps; d.growth = a.growth;
+  d.nesterov = a.nesterov; d.eps = a.eps; d.growth = a.growth; d.parts = a.parts;
   auto with = [&](const NsItem* items, int total) {
     NsDev x = d;
     x.items = items;
@@ -738,7 +803,7 @@ void muon_step(const MuonArgs& a, void* ws, hipStream_t stream) {
     d.step = k;
     d.last = k == a.steps - 1;
     d.co = a.coeffs[k];
-    product<NS_GRAM>("muon_gram", with(a.items_sym, a.n_sym), kMuonTile, stream);
+    gram_in_parts("muon_gram_part", "muon_gram_join", with(a.items_gram, a.n_gram), with(a.items_join, a.n_sym), stream);
     product<NS_POLY>("muon_poly", with(a.items_sym, a.n_sym), kMuonTile, stream);
     product<NS_APPLY>("muon_apply", with(a.items_apply, a.n_apply), kMuonTile, stream);
   }

@@ -1299,14 +1299,15 @@ class MuonTables:
     def __init__(self, matrices, vectors, device):
         require()
         h = hip()
-        assert self.MAT.itemsize == h.NS_MAT_BYTES
+        assert self.MAT.itemsize == h.NS_MAT_BYTES and h.NS_ITEM_BYTES == 24
         mats = np.zeros(len(matrices), dtype=self.MAT)
-        flat, small, out, split, sym, apply, floats, tile = [], [], [], [], [], [], 0, h.MUON_TILE
+        flat, small, out, split, gram, join, sym, apply, floats, tile = [], [], [], [], [], [], [], [], 0, h.MUON_TILE
+        shapes = [h.ns_shape(rows, cols) for _, rows, cols in matrices]
+        tiles_of = [0 if s[9] else (lambda t: t * (t + 1) // 2)(-(-s[2] // tile)) for s in shapes]   # of X X^T, lower triangle
         for i, (off, rows, cols) in enumerate(matrices):
-            r, c, rp, cp, tall, parts, chunk, sx, need, is_small = h.ns_shape(rows, cols)
+            r, c, rp, cp, tall, parts, chunk, sx, need, is_small = shapes[i]
             mats[i] = (off, off, cols, cols, floats, rows, cols, r, c, rp, cp, tall, parts, chunk, sx, math.sqrt(max(1.0, cols / rows)), 0)
             floats += (need + 63) // 64 * 64
-            tr, tc = -(-rp // tile), -(-cp // tile)
             flat += [(i, k) for k in range(parts)]
             blocks = [(i, k) for k in range((rp // 32) * (cp // 32))]
             if is_small:
@@ -1314,21 +1315,31 @@ class MuonTables:
                 out += blocks
                 continue
             split += blocks
-            sym += [(i, k) for k in range(tr * (tr + 1) // 2)]
-            apply += [(i, k) for k in range(tr * tc)]
+            sym += [(i, k) for k in range(tiles_of[i])]
+            apply += [(i, k) for k in range(-(-rp // tile) * -(-cp // tile))]
+            n = h.ns_splits(rows, cols, sum(tiles_of))
+            first = len(gram)
+            gram += [(i, k, cp // 32 * s // n, cp // 32 * (s + 1) // n - cp // 32 * s // n, first + k * n + s) for s in range(n) for k in range(tiles_of[i])]
+            join += [(i, k, 0, n, first + k * n) for k in range(tiles_of[i])]
         for off, n in vectors:
             if off % h.MUON_VEC_ALIGN:
                 raise ValueError("MuonTables: vectors start on multiples of 64 elements")
             for k in range(0, n, h.MUON_VEC_CHUNK):
                 flat.append((-1 - min(h.MUON_VEC_CHUNK, n - k), (off + k) // h.MUON_VEC_ALIGN))
-        self.workspace = torch.empty(max(1, floats), device=device, dtype=torch.float32)
+        self._parts = floats
+        self.workspace = torch.empty(max(1, floats + len(gram) * tile * tile), device=device, dtype=torch.float32)
         self._mats = torch.from_numpy(mats.view(np.uint8).copy()).to(device)
-        self._items = [torch.tensor(x, dtype=torch.int32).reshape(-1, 2).to(device) for x in (flat, small, out + split, sym, apply)]
+        self._items = {}
+        for name, items in (("flat", flat), ("small", small), ("split", out + split), ("gram", gram), ("join", join), ("sym", sym), ("apply", apply)):
+            table = np.zeros((len(items), 6), dtype=np.int32)
+            if items:
+                table[:, :len(items[0])] = items
+            self._items[name] = torch.from_numpy(table).to(device)
         self._out = len(out)
 
     def launch_args(self) -> dict:
-        d = dict(mats=self._mats.data_ptr(), ws=self.workspace.data_ptr(), n_out=self._out)
-        for name, t in zip(("flat", "small", "split", "sym", "apply"), self._items):
+        d = dict(mats=self._mats.data_ptr(), ws=self.workspace.data_ptr(), parts=self.workspace.data_ptr() + 4 * self._parts, n_out=self._out)
+        for name, t in self._items.items():
             d["items_" + name], d["n_" + name] = t.data_ptr(), t.shape[0]
         return d
 
