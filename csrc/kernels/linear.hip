@@ -110,8 +110,8 @@ void check_ws(const char* what, size_t need, const void* ws, size_t have) {
 int dz_rows(int M, int N) {
   if (M <= 0 || N <= 0) return 16;
   const int col_blocks = ceil_div(N, 256);
-  int blocks = ceil_div(1024, col_blocks);
-  if (blocks > 64) blocks = 64;
+  int blocks = ceil_div(2048, col_blocks);
+  if (blocks > 128) blocks = 128;
   int rows = ceil_div(M, blocks);
   return rows < 16 ? 16 : rows;
 }

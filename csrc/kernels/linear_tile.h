@@ -402,16 +402,27 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinDzArgs a) {
   const int m_begin = blockIdx.y * a.rows_per_block, m_end = min(a.M, m_begin + a.rows_per_block);
   floatx4 s = {0.f, 0.f, 0.f, 0.f};
   if (have > 0) {
-    for (int m = m_begin + wave; m < m_end; m += 4) {
-      floatx4 v = lin_load4<KIND>(a.dy, (long long)m * a.lddy + n, a.vec, have);
-      if (a.act != ACT_NONE) {
-        const floatx4 z = lin_load4<KIND>(a.pre, (long long)m * a.ldp + n, a.vec, have);
+    constexpr int U = 2;   // rows whose loads are in flight together
+    for (int m0 = m_begin + wave; m0 < m_end; m0 += 4 * U) {
+      floatx4 v[U], z[U];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < have) v[i] *= lin_act_grad<KIND>(a.act, z[i]);
+      for (int u = 0; u < U; ++u) {
+        const int m = min(m0 + 4 * u, m_end - 1);
+        v[u] = lin_load4<KIND>(a.dy, (long long)m * a.lddy + n, a.vec, have);
+        if (a.act != ACT_NONE) z[u] = lin_load4<KIND>(a.pre, (long long)m * a.ldp + n, a.vec, have);
       }
-      if (a.dz) lin_store4<KIND>(a.dz, (long long)m * a.lddz + n, 1, 4, v);   // zeros past N
-      s += v;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int m = m0 + 4 * u;
+        if (m >= m_end) break;
+        if (a.act != ACT_NONE) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < have) v[u][i] *= lin_act_grad<KIND>(a.act, z[u][i]);
+        }
+        if (a.dz) lin_store4<KIND>(a.dz, (long long)m * a.lddz + n, 1, 4, v[u]);   // zeros past N
+        s += v[u];
+      }
     }
   } else if (a.dz && n < a.lddz) {
     for (int m = m_begin + wave; m < m_end; m += 4) lin_store4<KIND>(a.dz, (long long)m * a.lddz + n, 1, 4, s);
@@ -461,18 +472,25 @@ struct LinColSumArgs { const float* part; long long N4; int blocks, N, accumulat
 template <MmKind KIND>
 __global__ __launch_bounds__(256) void linear_colsum_kernel(LinColSumArgs a) {
   DTF_ABORT_GUARD(a);
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= a.N) return;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  int b = 0;
-  for (; b + 4 <= a.blocks; b += 4) {
+  // 64 columns a workgroup; a wave adds every fourth block's sums, eight loads in flight, and the waves are added in order
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (n < a.N) {
+    for (int b = wave; b < a.blocks; b += 32) {
+      float v[8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) s[u] += a.part[(long long)(b + u) * a.N4 + n];
+      for (int u = 0; u < 8; ++u) v[u] = a.part[(long long)min(b + 4 * u, a.blocks - 1) * a.N4 + n];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += b + 4 * u < a.blocks ? v[u] : 0.f;
+    }
   }
-  for (; b < a.blocks; ++b) s[0] += a.part[(long long)b * a.N4 + n];
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave || n >= a.N) return;
   using E = typename MmElem<KIND>::type;
   E* out = reinterpret_cast<E*>(a.db) + n;
-  float v = (s[0] + s[1]) + (s[2] + s[3]);
+  float v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
   if (a.accumulate) v += (float)*out;
   *out = (E)v;
 }
@@ -571,7 +589,7 @@ LinLaunch lin_make_launch() {
   l.dz = [](const LinDzArgs& a, dim3 grid, hipStream_t s) { launch("linear_dz", linear_dz_kernel<KIND>, grid, dim3(256), 0, s, a); };
   l.pad = [](const LinPadArgs& a, hipStream_t s) { launch("linear_pad", linear_pad_kernel<KIND>, dim3(1024, 2), dim3(256), 0, s, a); };
   l.colsum = [](const LinColSumArgs& a, hipStream_t s) {
-    launch("linear_colsum", linear_colsum_kernel<KIND>, dim3((unsigned)ceil_div(a.N, 256)), dim3(256), 0, s, a);
+    launch("linear_colsum", linear_colsum_kernel<KIND>, dim3((unsigned)ceil_div(a.N, 64)), dim3(256), 0, s, a);
   };
   return l;
 }
