@@ -61,7 +61,7 @@ __device__ __forceinline__ void mm_mfma_all(const Frag& x, const Frag& y, floatx
 
 // 16 bytes per lane from memory to LDS at lds + 16 lane, past the registers; done when vmcnt says so. Written in asm
 // because the compiler, which cannot tell the two stages of a double buffer apart, would wait for every such load
-// before the next read of LDS. There is no output register.
+// before the next read of LDS. There is no output register; M0 is written in the same block and has no other use here.
 __device__ __forceinline__ void lds_load16(const char* base, unsigned off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory");
 }

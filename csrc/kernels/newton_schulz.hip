@@ -394,7 +394,7 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
   }
   // The output, in G's orientation: a lane holds four consecutive elements of a row of it.
   const float tau = tau_at(a.ws[m.ws + 2 * kNsNormParts], a.growth, a.step + 1);
-  const float f = tau / (kScaleP * m.sx);
+  const float f = 1.f / (kScaleP * m.sx);   // tau apart: their product can leave fp32's normal range
   const float lr = a.m ? a.hyper[0] * m.scale : 0.f, decay = a.m ? a.hyper[3] : 0.f;
 #pragma unroll
   for (int i = 0; i < MI; ++i)
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
       if (row >= m.rows) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (col + e < m.cols) ns_write(a, m, row, col + e, acc[i][j][e] * f, lr, decay);
+        if (col + e < m.cols) ns_write(a, m, row, col + e, acc[i][j][e] * f * tau, lr, decay);
     }
 }
 
@@ -644,13 +644,13 @@ __global__ __launch_bounds__(256) void ns_out_kernel(NsDev a) {
     }
   }
   __syncthreads();
-  const float f = a.ws[m.ws + 2 * kNsNormParts] / m.sx;
+  const float f = 1.f / m.sx, tau = a.ws[m.ws + 2 * kNsNormParts];
   const float lr = a.m ? a.hyper[0] * m.scale : 0.f, decay = a.m ? a.hyper[3] : 0.f;
   const int r0 = (m.tall ? bj : bi) * 32, c0 = (m.tall ? bi : bj) * 32;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int y = (threadIdx.x >> 5) + 8 * k, x = threadIdx.x & 31;
-    if (r0 + y < m.rows && c0 + x < m.cols) ns_write(a, m, r0 + y, c0 + x, block[y][x] * f, lr, decay);
+    if (r0 + y < m.rows && c0 + x < m.cols) ns_write(a, m, r0 + y, c0 + x, block[y][x] * f * tau, lr, decay);
   }
 }
 

@@ -1083,20 +1083,28 @@ def _span(t: torch.Tensor) -> tuple:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether two tensors of a call share memory. Column ranges of one buffer do not, though their spans do."""
+    (lo, hi), (a, b) = _span(s), _span(t)
+    if not (a < hi and lo < b):
+        return False
+    if s.dim() == 2 and t.dim() == 2 and s.shape[0] > 1 and t.shape[0] > 1 and s.stride(0) == t.stride(0) and s.dtype == t.dtype:
+        ld, size = s.stride(0), s.element_size()
+        if ld > 0 and (lo - a) % size == 0:
+            at = (lo - a) // size % ld   # where s begins in the rows of t
+            return not (at >= t.shape[1] and at + s.shape[1] <= ld)
+    return True
+
+
 def _check_apart(what: str, written, read, in_place=()) -> None:
-    """Refuses an output that overlaps an input or another output; `in_place` tensors may be an output itself."""
+    """Refuses an output that overlaps an input or another output; `in_place` tensors may be the first output itself."""
     outs = [t for t in written if t is not None]
     for i, o in enumerate(outs):
-        lo, hi = _span(o)
         for t in [r for r in read if r is not None] + outs[i + 1:]:
-            a, b = _span(t)
-            if a < hi and lo < b:
+            if _overlap(o, t):
                 raise ValueError(f"{what}: an output overlaps another tensor of the call")
         for t in in_place:
-            if t is None:
-                continue
-            a, b = _span(t)
-            if a < hi and lo < b and not (o is outs[0] and t.data_ptr() == o.data_ptr() and t.stride() == o.stride()):
+            if t is not None and _overlap(o, t) and not (o is outs[0] and t.data_ptr() == o.data_ptr() and t.stride() == o.stride()):
                 raise ValueError(f"{what}: an output overlaps another tensor of the call")
 
 
@@ -1124,7 +1132,7 @@ def linear(x, w, bias=None, *, activation: str = "none", residual=None, trans_w:
     type, float32, bfloat16 or float16; sums are fp32 (float32 products run on the exact fp32 matrix pipe) and every
     output is rounded once. Matrices may be row-strided views. activation: none, relu, gelu (erf), gelu_tanh, silu.
     pre [M,N] receives x W + bias for linear_bwd. out may be `residual` itself, otherwise outputs overlap nothing.
-    workspace: linear_workspace() bytes; a call recorded into a step program has to bring its own."""
+    workspace: linear_workspace() bytes; a call recorded into a step program has to bring its own. Not differentiated by autograd."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"linear: unknown activation {activation!r}")
@@ -1351,6 +1359,8 @@ def muon_step(p, g, m, v, hyper, tables: MuonTables, *, nesterov: bool, steps: i
     n = p.numel()
     if g.numel() != n or m.numel() != n or v.numel() != n or hyper.numel() < HYPER_SLOTS:
         raise ValueError("muon_step: size mismatch")
+    if any(t.get_device() != torch.cuda.current_device() for t in (p, g, m, v, hyper, tables.workspace)):
+        raise ValueError("muon_step: the buffers are not on the current device")
     flat, growth = _ns_steps(_ns_key(coeffs), steps)
     hip().muon_step(dict(p=_chk(p, "p"), g=_chk(g, "g"), m=_chk(m, "m"), v=_chk(v, "v"), hyper=_chk(hyper, "hyper"), nesterov=int(nesterov),
                          coeffs=flat, growth=growth, eps=float(eps), **tables.launch_args()), stream())

@@ -97,6 +97,38 @@ def test_linear_shapes(m, k, n, trans_w, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("m,k,n", [(4090, 200, 4088), (2000, 136, 2040), (4089, 77, 4093), (520, 8200, 136), (70, 20000, 65), (4, 8192, 1000), (1, 70000, 24),
+                                   (3, 16, 9000), (8, 4096, 72)])
+def test_linear_large(m, k, n, trans_w, dtype):
+    """Every tile, split k, padded copies and the few-rows kernels, with edges; forward and gradients."""
+    x, w, bias, res = make(m, k, n, dtype, trans_w, seed=12)
+    pre = torch.empty(m, n, device="cuda", dtype=dtype)
+    y = nv.linear(x, w, bias, activation="silu", residual=res, trans_w=trans_w, pre=pre)
+    check_forward(x, w, bias, res, "silu", trans_w, y, pre)
+    check_backward(res, x, w, pre, "silu", trans_w, *nv.linear_bwd(res, x, w, pre=pre, activation="silu", trans_w=trans_w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ld", [(1 << 22) - 8, (1 << 24) + 8, (1 << 22) + 3])
+def test_linear_rows_far_apart(ld):
+    """Rows whose addresses pass 2^31 and 2^32 bytes, read and written, below and above the stride that one 32-bit offset covers."""
+    m, k, n = 270 if ld < 1 << 23 else 140, 72, 40
+    x, w, bias, res = make(m, k, n, torch.bfloat16, False, seed=13)
+    big = torch.empty(m * ld, device="cuda", dtype=torch.bfloat16)
+    far = big.view(m, ld)
+    xf, yf, zf = far[:, :k], far[:, 100:100 + n], far[:, 200:200 + n]
+    xf.copy_(x)
+    nv.linear(xf, w, bias, activation="relu", residual=res, out=yf, pre=zf)
+    check_forward(x, w, bias, res, "relu", False, yf, zf)
+    dyf, dxf = far[:, 300:300 + n], far[:, 400:400 + k]
+    dyf.copy_(res)
+    dx, dw, db = nv.linear_bwd(dyf, xf, w, pre=zf, activation="relu", dx=dxf)
+    check_backward(res, x, w, zf, "relu", False, dxf, dw, db)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("act", ACTS)
 def test_linear_activations(act, dtype):
     x, w, bias, _ = make(40, 96, 56, dtype, False, seed=1)
@@ -365,6 +397,11 @@ def test_linear_refuses_bad_arguments():
     out = f(4, 5)
     with pytest.raises(ValueError):
         nv.linear(x, w, residual=f(5 * 5)[2:22].view(4, 5), out=out, pre=out)
+    wide = f(4, 20)
+    assert not nv._overlap(wide[:, :6], wide[:, 6:11]) and not nv._overlap(wide[:, 6:11], wide[:, :6]) and not nv._overlap(wide[:, 15:], wide[1:, :15])
+    assert nv._overlap(wide[:, :7], wide[:, 6:11]) and nv._overlap(wide[:, 2:4], wide[:, :20]) and nv._overlap(wide[1:, :6], wide[:, :6])
+    with pytest.raises(ValueError):
+        nv.linear(wide[:, :6], w, out=wide[:, 5:10])
     buf = f(40)
     with pytest.raises(ValueError):
         nv.linear(x, w, residual=buf[0:20].view(4, 5), out=buf[10:30].view(4, 5))

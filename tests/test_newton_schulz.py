@@ -25,7 +25,8 @@ DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 def ns64(g, steps=5, coeffs=ref.NS_COEFFS, eps=1e-7):
     """(result, error bound in the Frobenius norm before the output's rounding)"""
     per = [coeffs] * steps if not isinstance(coeffs[0], (tuple, list)) else list(coeffs)
-    x = g.double().cpu()
+    x = g.double()
+    x = x if x.numel() > 1 << 20 else x.cpu()
     tall = x.shape[0] > x.shape[1]
     x = x.t() if tall else x
     r, c = x.shape
@@ -40,7 +41,7 @@ def ns64(g, steps=5, coeffs=ref.NS_COEFFS, eps=1e-7):
         m = x @ x.t()
         x = a * x + (b * m + cc * m @ m) @ x
         err = lip * err + eta * float(x.norm())
-    return (x.t() if tall else x), err
+    return (x.t() if tall else x).cpu(), err
 
 
 def check(out, g, steps=5, coeffs=ref.NS_COEFFS, eps=1e-7):
@@ -74,6 +75,16 @@ def test_newton_schulz_shapes(m, n, dtype):
     out = nv.newton_schulz(g)
     assert out.shape == g.shape and out.dtype == dtype and torch.equal(g, keep)
     check(out, g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,dtype", [(1500, 2600, torch.float32), (2600, 1111, torch.float16), (2048, 2050, torch.float32), (4090, 4000, torch.float32),
+                                       (1024, 4096, torch.bfloat16), (130, 9000, torch.float32), (9000, 100, torch.bfloat16), (3, 40000, torch.float32),
+                                       (769, 64, torch.float32), (768, 64, torch.float32), (32, 1024, torch.float32), (1025, 32, torch.float32)])
+def test_newton_schulz_large(m, n, dtype):
+    """The larger tiles, the split X X^T, and both sides of the border of the one-workgroup kernel."""
+    g = gradient(m, n, seed=3, scale=1.0).to(dtype).cuda()
+    check(nv.newton_schulz(g), g)
 
 
 @pytest.mark.gpu
@@ -117,10 +128,10 @@ def test_newton_schulz_strided_and_in_place(dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("scale", [1e18, 1e3, 1e-6, 1e-9, 1e-12, 1e-20, 1e-34])
+@pytest.mark.parametrize("scale", [1e18, 1e3, 1e-6, 1e-9, 1e-12, 1e-20, 1e-34, 1e-38])
 def test_newton_schulz_norms_far_from_one(scale):
     """Squares leave fp32's range on both sides; far below eps the result is the linear part, far below one."""
-    for m, n in ((40, 72), (96, 64)):
+    for m, n in ((40, 72), (96, 64), (130, 200), (300, 140)):
         g = (gradient(m, n, seed=4, scale=1.0) * scale).cuda()
         check(nv.newton_schulz(g), g)
 
