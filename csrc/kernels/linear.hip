@@ -62,7 +62,7 @@ Plan plan_of(const MmProduct& p) {
   const int line_a = p.kc_a ? p.K : p.M, line_b = p.kc_b ? p.K : p.N;
   const bool ok_a = direct(p.a, p.lda, line_a, p.pad_a), ok_b = direct(p.b, p.ldb, line_b, p.pad_b);
   bool whole = ok_a && ok_b;
-  // One that is not is copied where the product reads it often enough (fp16 1003 x 1531 x 2050: 35 -> 22 us)
+  // One that is not is copied where the product reads it often enough (fp16 gradients of 777 x 1001 x 1300: 97 -> 45 us)
   if (!whole && p.M >= 64 && p.N >= 64 && p.K >= 64 && line_a < (1 << 20) && line_b < (1 << 20)) {
     if (!ok_a) { l.copy_a = 1; l.ld_a = (line_a + epc - 1) / epc * epc; l.bytes_a = round_up((size_t)l.ld_a * (p.kc_a ? p.M : p.K) * es); }
     if (!ok_b) { l.copy_b = 1; l.ld_b = (line_b + epc - 1) / epc * epc; l.bytes_b = round_up((size_t)l.ld_b * (p.kc_b ? p.N : p.K) * es); }

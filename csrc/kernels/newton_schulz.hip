@@ -751,7 +751,7 @@ void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t strea
     launch("ns_out", ns_out_kernel, dim3(s.total), dim3(256), 0, stream, s);
     return;
   }
-  // X X^T of few rows and many columns: in parts, which are added in order (us of 512 x 3136 26 -> 13, of 1024 x 4096 36 -> 22)
+  // X X^T of few rows and many columns: in parts, which are added in order (us of 512 x 3136 26 -> 15, of 1024 x 4096 36 -> 26)
   const int splits = gram_splits(m, a.batch);
   d.splits = splits;
   d.parts = d.ws + ns_floats(m) * a.batch;
