@@ -53,6 +53,8 @@ __device__ __forceinline__ float lin_act(int act, float z) {
 template <MmKind KIND>
 __device__ __forceinline__ float lin_act_grad(int act, float z) {
   float gauss;
+  // Every slope has reached its limit long before: no z^2 that overflows and no infinity times zero. NaN stays.
+  z = z > 1e4f ? 1e4f : z < -1e4f ? -1e4f : z;
   switch (act) {
     case ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case ACT_GELU: {

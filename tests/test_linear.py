@@ -271,6 +271,25 @@ def test_linear_bwd_strided_accumulating(pad, shift, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS[1:])
+def test_linear_bwd_slopes_far_out(act, dtype):
+    """Pre-activations far from zero, up to infinity: the slope is 0 or 1 to the last bit, and NaN stays NaN."""
+    far = [300.0, 65504.0, 1e20, 3e38, float("inf")]
+    pre = torch.tensor([far, [-v for v in far]], dtype=torch.float64).to(dtype).cuda()
+    dy = torch.full((2, 5), 2.0, dtype=dtype, device="cuda")
+    eye = torch.eye(5, dtype=dtype, device="cuda")
+    x = torch.ones(2, 3, dtype=dtype, device="cuda")
+    dx, dw, db = nv.linear_bwd(dy, x, eye[:3].contiguous(), pre=pre, activation=act)
+    assert torch.equal(dx, torch.tensor([[2.0] * 3, [0.0] * 3], dtype=dtype, device="cuda"))
+    assert torch.equal(db, torch.full((5,), 2.0, dtype=dtype, device="cuda")) and torch.equal(dw, torch.full((3, 5), 2.0, dtype=dtype, device="cuda"))
+    if act != "relu":
+        pre[0, 1] = float("nan")
+        db = nv.linear_bwd(dy, x, eye[:3].contiguous(), pre=pre, activation=act)[2]
+        assert db.isnan().tolist() == [False, True, False, False, False]
+
+
+@pytest.mark.gpu
 def test_linear_gradients_against_differences():
     """Directional derivatives of sum(c * y) by central differences in 64 bits against the fp32 kernels' gradients."""
     m, k, n = 12, 20, 9
