@@ -52,8 +52,18 @@ int pick_tile(const MmProduct& p) {
   }
   return best;
 }
+// Sizes and indices of a tile or a stage past a dimension's end are 32 bits.
+void check_sizes(long long M, long long N, long long K) {
+  constexpr long long most = (1ll << 31) - 65536;
+  if (M > most || N > most || K > most) throw std::runtime_error("linear: a dimension passes 2^31 - 65536");
+}
+// A launch has fewer than 2^32 threads.
+void check_blocks(long long blocks, int threads) {
+  if (blocks * threads > 0xffffffffll) throw std::runtime_error("linear: the product has too many tiles");
+}
 Plan plan_of(const MmProduct& p) {
   Plan l{};
+  check_sizes(p.M, p.N, p.K);
   const int es = elem_bytes(p.kind), epc = 16 / es;
   // An operand can be loaded 16 bytes at a time if its lines start and end on multiples of them
   auto direct = [&](const void* base, long long ld, int contiguous, int padded) {
@@ -82,6 +92,7 @@ Plan plan_of(const MmProduct& p) {
     l.k_per_split = ceil_div(ceil_div(p.K, splits), 8) * 8;
     l.splits = ceil_div(p.K, l.k_per_split);
     l.bytes = l.splits > 1 ? round_up((size_t)l.splits * p.M * l.N4 * sizeof(float)) : 0;
+    check_blocks((long long)l.gx * l.splits + 7, 64 * kRowWaves);
     return l;
   }
   const int tile = kLinTiles[l.variant].t;
@@ -99,6 +110,7 @@ Plan plan_of(const MmProduct& p) {
   l.splits = p.K > 0 ? ceil_div(p.K, per) : 1;
   l.k_per_split = p.K > 0 ? per : kb;
   l.bytes = l.splits > 1 ? round_up((size_t)l.splits * p.M * l.N4 * sizeof(float)) : 0;
+  check_blocks(tiles * l.splits + 7, 64 * kLinTiles[l.variant].wgm * kLinTiles[l.variant].wgn);
   return l;
 }
 
@@ -128,7 +140,6 @@ void mm_product(const MmProduct& p, void* ws, size_t ws_bytes, hipStream_t strea
   if (p.M <= 0 || p.N <= 0) return;
   const Plan l = plan_of(p);
   check_ws("linear", l.bytes + l.bytes_a + l.bytes_b, ws, ws_bytes);
-  if ((long long)l.gx * l.gy * l.splits > 0x3fffffff) throw std::runtime_error("linear: the product has too many tiles");
   LinTileArgs a{};
   a.p = p;
   a.partial = reinterpret_cast<float*>(ws);
@@ -182,6 +193,8 @@ struct BwdPlan {
 };
 BwdPlan bwd_plan(const LinearBwdArgs& a, void* dz) {
   BwdPlan b{};
+  check_sizes(a.M, a.N, a.K);
+  if (a.db) check_blocks(ceil_div(a.N, 64), 256);
   const bool own_dz = a.act != ACT_NONE && (a.dx || a.dw);
   b.N4 = ((long long)a.N + 3) / 4 * 4;
   b.lddz = ((long long)a.N + 7) / 8 * 8;

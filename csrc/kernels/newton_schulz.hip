@@ -689,10 +689,13 @@ int apply_tiles(const NsMat& m, int T) { return ceil_div(m.rp, T) * ceil_div(m.c
 void ns_shape(NsMat& m, int rows, int cols) {
   m.rows = rows; m.cols = cols;
   m.tall = rows > cols;
+  if (rows > (1 << 30) || cols > (1 << 30)) throw std::runtime_error("newton_schulz: a dimension passes 2^30");
   m.r = rows < cols ? rows : cols;
   m.c = rows < cols ? cols : rows;
   m.rp = ceil_div(m.r, 32) * 32;
   m.cp = ceil_div(m.c, 32) * 32;
+  // the rows of a tile are found by 32-bit byte offsets from its first
+  if ((long long)(m.rp < 256 ? m.rp : 256) * m.cp > 1ll << 30) throw std::runtime_error("newton_schulz: the rows are too long");
   const long long n = (long long)rows * cols;
   const long long chunk = (n + kNsNormParts - 1) / kNsNormParts;
   m.chunk = (int)(((chunk < 2048 ? 2048 : chunk) + 63) / 64 * 64);
@@ -732,7 +735,7 @@ void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t strea
   d.eps = a.eps; d.growth = a.growth;
   const NsMat& m = d.one;
   auto with = [&](int per) {
-    if ((long long)per * a.batch > 0x3fffffff) throw std::runtime_error("newton_schulz: too many tiles");
+    if ((long long)per * a.batch > 0x7ffff8) throw std::runtime_error("newton_schulz: too many tiles");   // x 512 threads: below 2^32
     NsDev x = d;
     x.per_mat = per;
     x.total = per * a.batch;

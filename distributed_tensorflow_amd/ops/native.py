@@ -1049,8 +1049,8 @@ def _mat(t: torch.Tensor, what: str, like: torch.Tensor, rows: int, cols: int, w
         raise ValueError(f"{what}: the elements of a row must be contiguous")
     if written and ld < cols:
         raise ValueError(f"{what}: rows overlap")
-    if rows >= 2**31 or cols >= 2**31:
-        raise ValueError(f"{what}: a dimension passes 2^31")
+    if rows > 2**31 - 65536 or cols > 2**31 - 65536:
+        raise ValueError(f"{what}: a dimension passes 2^31 - 65536")
     return t.data_ptr(), ld
 
 

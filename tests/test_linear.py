@@ -441,3 +441,19 @@ def test_linear_workspace_refusals():
         nv._workspace("linear", 8, ok[1:], dev)
     with pytest.raises(ValueError):
         nv._workspace("linear", 8, ok[::2], dev)
+
+
+def test_linear_refuses_sizes_past_its_indices():
+    """Dimensions that a tile's 32-bit indices or a launch's threads could not count: refused when the workspace is asked for."""
+    if nv._hip is None:
+        pytest.skip("extension not built")
+    top = 2 ** 31
+    for m, n, k in ((top - 1, 1, 1), (1, top - 1, 1), (1, 1, top - 1), (top - 65536, 512, 8), (512, top - 65536, 8)):
+        with pytest.raises(RuntimeError, match="dimension|too many tiles"):
+            nv.linear_workspace(m, n, k)
+    with pytest.raises(RuntimeError, match="too many tiles"):   # 16 columns a workgroup of 1024 threads
+        nv.linear_workspace(1, 2 ** 27, 8, torch.bfloat16, trans_w=True)
+    with pytest.raises(RuntimeError, match="too many tiles"):   # column sums, 64 columns a workgroup of 256
+        nv.linear_bwd_workspace(1, 2 ** 30, 1)
+    with pytest.raises(RuntimeError, match="dimension"):
+        nv.linear_bwd_workspace(1, top - 1, 1)

@@ -207,6 +207,16 @@ def test_newton_schulz_refuses_bad_arguments():
             call()
 
 
+def test_newton_schulz_refuses_sizes_past_its_indices():
+    """32-bit offsets inside a tile: rows x 4-byte elements of up to 256 rows have to stay within 2^32."""
+    if nv._hip is None:
+        pytest.skip("extension not built")
+    assert nv.newton_schulz_workspace(32, 2 ** 25) > 0 and nv.newton_schulz_workspace(2 ** 22, 256) > 0
+    for m, n in ((65, 2 ** 24), (2 ** 24, 65), (32, 2 ** 25 + 1), (256, 2 ** 22 + 1), (1, 2 ** 30 + 1), (2 ** 31 - 1, 1)):
+        with pytest.raises(RuntimeError, match="too long|dimension"):
+            nv.newton_schulz_workspace(m, n)
+
+
 def test_growth_bounds_the_sequence():
     """The accepted sequences keep singular values within 3.8 (brute force over a fine grid)."""
     for coeffs in (ref.NS_COEFFS, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (4.0848, -6.8946, 2.927)):
