@@ -5,13 +5,14 @@
 // stored pre-activation, the activation and the residual cost their own bytes and no launch. The backward pass
 // is one pass over dy and the pre-activation (dz and the column sums) and two products.
 #include "linear_tile.h"
+#include <math.h>
 
 namespace dtf {
 namespace {
 
-// Rows that the few-rows kernels take. More go through 64 x 64 tiles: 4096 x 4096, us by rows kernel / tiles, bf16 W [K,N] 1 row
-// 10.3 / 17, 4 rows 13.3 / 13.7, 8 rows (spills) 37 / 13.7; fp32 8 rows 18.3 / 25.9.
-constexpr int lin_rows_max(int kind) { return kind == MM_F32 ? 8 : 4; }
+// Rows that the few-rows kernels take; more go through 32 x 64 tiles. 4096 x 4096, us by rows kernel / tiles: bf16 W [K,N] 1 row 10.6 / 9.7 (1024 x 1024
+// 5.2 / 6.5), 2 rows 12.0 / 9.9; W [N,K] 2 rows 8.6 / 9.9, 3 rows 10.6 / 9.9; fp32 W [K,N] 4 rows 16.6 / 20.1, 5 rows 18.7 / 20.2 (1024 x 1024 10.8 / 8.5).
+int lin_rows_max(const MmProduct& p) { return p.kind == MM_F32 ? 4 : p.kc_b ? 2 : 1; }
 constexpr size_t kMaxPartialBytes = 256ull << 20;   // partial sums of a split product
 
 const LinLaunch& lin_launch(int kind) {
@@ -33,23 +34,36 @@ struct Plan {
   long long ld_a, ld_b;          // leading dimension of the copy
   size_t bytes, bytes_a, bytes_b;   // partial sums, copies
 };
-// The larger the tile the less is loaded per product, but it takes about a tile per CU to use the card. The choice goes by an
-// estimate: rounds of workgroups times stages of k, with the us of a round's stage measured with half the CUs busy and with all
-// (whole products, us by 64 / 128 / 256: bf16 8192 x 4096 x 4096 383 / 298 / 216, 2048 cubed 28 / 22 / 39, 1024 x 1536 x 2048 12.6 / 14.7 / -;
-// fp32 2048 cubed 132 / 125 / 148).
-struct TileCost { int variant, slots; float some16, full16, some32, full32; };
-constexpr TileCost kTileCosts[] = {{LIN_64, 512, 0.22f, 0.39f, 0.6f, 1.0f}, {LIN_128, 256, 0.55f, 0.6f, 1.8f, 1.92f}, {LIN_256, 256, 1.5f, 1.63f, 7.0f, 7.2f}};
-int pick_tile(const MmProduct& p) {
-  int best = LIN_64;
-  float least = 0.f;
-  for (const TileCost& c : kTileCosts) {
-    const int t = kLinTiles[c.variant].t;
-    const float n = (float)((long long)ceil_div(p.M, t) * ceil_div(p.N, t)) / (float)c.slots;
-    // two workgroups share a CU with 64 x 64 tiles: a round need not be full; else every round begun takes its time
-    const float rounds = n <= 1.f ? 1.f : c.slots > 256 ? n + 0.25f : ceilf(n);
-    const float us = rounds * (n <= 0.6f ? (p.kind == MM_F32 ? c.some32 : c.some16) : (p.kind == MM_F32 ? c.full32 : c.full16));
-    if (c.variant == LIN_64 || us < least) { best = c.variant; least = us; }
+// The larger the tile the less is loaded per product, but it takes about a tile per CU to use the card; and k in parts fills it with fewer
+// tiles, for the price of the parts' way through memory and a second launch. The choice goes by an estimate of the time: what a
+// workgroup takes for a stage of 128 bytes of k, alone on its CU and with as many as fit, and what a launch takes besides, in us (fitted
+// to 1700 products of 9 to 8192 rows and columns, which it gives within 5 % (fp32) and 10 %; what it picks takes 1.6 % more than the best of
+// them, and 14 % less than tiles picked first and parts of at least twelve stages after).
+struct TileCost { int variant, per_cu; float alone, full, launch; };
+constexpr TileCost kTileCosts[2][4] = {
+    {{LIN_64, 2, 0.58f, 1.11f, 4.7f}, {LIN_128, 1, 1.8f, 1.87f, 5.9f}, {LIN_256, 1, 7.0f, 7.0f, 11.3f}, {LIN_32, 3, 0.33f, 0.89f, 4.4f}},   // fp32
+    {{LIN_64, 2, 0.24f, 0.5f, 4.3f}, {LIN_128, 1, 0.45f, 0.7f, 5.1f}, {LIN_256, 1, 1.22f, 1.32f, 9.7f}, {LIN_32, 3, 0.16f, 0.53f, 4.0f}}};  // 16 bits
+// Through registers, 128 x 128: fp32 and 16 bits
+constexpr TileCost kRegsCost[2] = {{LIN_REGS, 1, 2.6f, 3.f, 5.f}, {LIN_REGS, 1, 1.8f, 2.f, 5.f}};
+constexpr int kSplitChoices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 256};
+struct TilePick { int variant, splits; float us; };
+void pick_splits(const MmProduct& p, const TileCost& c, TilePick& best) {
+  const int stages = ceil_div(p.K, 128 / elem_bytes(p.kind));
+  const long long tiles = (long long)ceil_div(p.M, kLinTiles[c.variant].tm) * ceil_div(p.N, kLinTiles[c.variant].tn);
+  const float plane = (float)p.M * (float)p.N * 4.f;   // bytes of a part
+  for (int splits : kSplitChoices) {
+    if (splits > 1 && (stages < 2 * splits || tiles * splits > 2048 || plane * splits > (float)kMaxPartialBytes)) break;
+    const int per = ceil_div(stages, splits);
+    const float n = (float)((tiles * splits + 255) / 256);   // workgroups of the busiest CU
+    const float stage = c.per_cu > 1 ? fmaxf(c.alone, c.full * n / c.per_cu) : tiles * splits <= 154 ? c.alone : c.full * n;
+    const float us = c.launch + stage * per + (splits > 1 ? 0.8f + 0.25f * splits + splits * plane * 4e-7f : 0.f);
+    if (us < best.us) best = TilePick{c.variant, splits, us};
   }
+}
+TilePick pick_tile(const MmProduct& p) {
+  TilePick best{LIN_64, 1, 3e38f};
+  for (const TileCost& c : kTileCosts[p.kind != MM_F32])
+    if (c.variant != LIN_32 || (p.kc_a && p.M <= 256)) pick_splits(p, c, best);
   return best;
 }
 // Sizes and indices of a tile or a stage past a dimension's end are 32 bits.
@@ -72,16 +86,19 @@ Plan plan_of(const MmProduct& p) {
   const int line_a = p.kc_a ? p.K : p.M, line_b = p.kc_b ? p.K : p.N;
   const bool ok_a = direct(p.a, p.lda, line_a, p.pad_a), ok_b = direct(p.b, p.ldb, line_b, p.pad_b);
   bool whole = ok_a && ok_b;
-  // One that is not is copied where the product reads it often enough (fp16 gradients of 777 x 1001 x 1300: 97 -> 45 us)
-  if (!whole && p.M >= 64 && p.N >= 64 && p.K >= 64 && line_a < (1 << 20) && line_b < (1 << 20)) {
-    if (!ok_a) { l.copy_a = 1; l.ld_a = (line_a + epc - 1) / epc * epc; l.bytes_a = round_up((size_t)l.ld_a * (p.kc_a ? p.M : p.K) * es); }
-    if (!ok_b) { l.copy_b = 1; l.ld_b = (line_b + epc - 1) / epc * epc; l.bytes_b = round_up((size_t)l.ld_b * (p.kc_b ? p.N : p.K) * es); }
+  // One that is not is copied, unless its lines or the whole are very long: 128 x 128 tiles that load it as it is take a third longer at
+  // 1000 cubed (fp16 gradients of 777 x 1001 x 1300 97 us, 45 with copies), and 4 to 8 times as long for few rows (bf16 21 x 5904 x 225 19.5 and
+  // 13.4 us, fp32 1 x 973 x 628 14.7 and 11.8, the former in the best number of parts).
+  const int rows_a = p.kc_a ? p.M : p.K, rows_b = p.kc_b ? p.N : p.K;
+  auto copied = [&](int line, int rows) { return line < (1 << 20) && ((long long)line / epc + 1) * rows < (1 << 30); };
+  if (!whole && (ok_a || copied(line_a, rows_a)) && (ok_b || copied(line_b, rows_b))) {
+    if (!ok_a) { l.copy_a = 1; l.ld_a = (line_a + epc - 1) / epc * epc; l.bytes_a = round_up((size_t)l.ld_a * rows_a * es); }
+    if (!ok_b) { l.copy_b = 1; l.ld_b = (line_b + epc - 1) / epc * epc; l.bytes_b = round_up((size_t)l.ld_b * rows_b * es); }
     whole = true;
   }
-  l.variant = whole ? pick_tile(p) : LIN_REGS;
   const int kb = 128 / es;
   // A few rows: no tile is worth filling. x has to fit LDS where W's rows are along k.
-  if (whole && p.kc_a && p.M <= lin_rows_max(p.kind) && !(p.K & 7) && p.K > 0 && (!p.kc_b || (long long)8 * p.K * es <= 128 * 1024)) {
+  if (whole && p.kc_a && p.M <= lin_rows_max(p) && !(p.K & 7) && p.K > 0 && (!p.kc_b || (long long)4 * p.K * es <= 128 * 1024)) {
     l.variant = LIN_ROWS;
     l.N4 = ((long long)p.N + 3) / 4 * 4;
     l.gx = p.kc_b ? ceil_div(p.N, kRowWaves) : ceil_div(p.N, lin_row_lanes(p.N, 16 / es) * (16 / es));
@@ -95,18 +112,15 @@ Plan plan_of(const MmProduct& p) {
     check_blocks((long long)l.gx * l.splits + 7, 64 * kRowWaves);
     return l;
   }
-  const int tile = kLinTiles[l.variant].t;
-  l.gx = ceil_div(p.N, tile);
-  l.gy = ceil_div(p.M, tile);
+  TilePick pick{LIN_REGS, 1, 3e38f};
+  if (whole) pick = pick_tile(p);
+  else pick_splits(p, kRegsCost[p.kind != MM_F32], pick);
+  l.variant = pick.variant;
+  l.gx = ceil_div(p.N, kLinTiles[l.variant].tn);
+  l.gy = ceil_div(p.M, kLinTiles[l.variant].tm);
   l.N4 = ((long long)p.N + 3) / 4 * 4;
-  // Few tiles and a long k: several workgroups share a tile's k, twelve stages each at least, until two stand on every CU
-  // (fp32 128 x 3136 x 512, 64 x 64 tiles, us in 1 / 4 / 8 / 16 parts: 40 / 22.4 / 19.0 / 18.8, the host's time).
   const long long tiles = (long long)l.gx * l.gy;
-  const int stages = ceil_div(p.K, kb);
-  const int slots = l.variant == LIN_REGS || l.variant == LIN_64 ? 512 : 256;
-  int splits = 1;
-  while (tiles * splits * 2 <= slots && stages >= splits * 24 && (size_t)p.M * l.N4 * splits * 8 <= kMaxPartialBytes) splits *= 2;
-  const int per = ceil_div(stages, splits) * kb;
+  const int per = ceil_div(ceil_div(p.K, kb), pick.splits) * kb;
   l.splits = p.K > 0 ? ceil_div(p.K, per) : 1;
   l.k_per_split = p.K > 0 ? per : kb;
   l.bytes = l.splits > 1 ? round_up((size_t)l.splits * p.M * l.N4 * sizeof(float)) : 0;
@@ -148,7 +162,7 @@ void mm_product(const MmProduct& p, void* ws, size_t ws_bytes, hipStream_t strea
   a.gx = l.gx; a.gy = l.gy; a.splits = l.splits; a.total = l.gx * l.gy * l.splits;
   const int es = elem_bytes(p.kind), epc = 16 / es, v4 = 4 * es;
   auto up = [&](int n) { return (n + epc - 1) / epc * epc; };
-  if (l.copy_a || l.copy_b) {
+  if ((l.copy_a || l.copy_b) && p.K > 0) {
     LinPadArgs c{};
     char* at = reinterpret_cast<char*>(ws) + l.bytes;
     if (l.copy_a) {

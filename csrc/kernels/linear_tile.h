@@ -176,7 +176,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tile_kernel(LinTileArgs
   // tensors are read and written 64 columns at once and the epilogue's code exists once. Each wave has its own rows: no barrier.
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, l15 = lane & 15;
   const int wm = (wave / WGN) * (BM / WGM), wn = (wave % WGN) * (BN / WGN);
-  constexpr int PITCH = LinEpilogue<NJ>::PITCH, LANES = NJ * 4, RSTEP = 64 / LANES, U = 4;   // lanes to a row, rows at once, reads ahead
+  constexpr int PITCH = LinEpilogue<NJ>::PITCH, LANES = NJ * 4, RSTEP = 64 / LANES, U = RSTEP > 8 ? 32 / RSTEP : 4;   // lanes to a row, rows at once, reads ahead
   static_assert(64 % LANES == 0 && 32 % (RSTEP * U) == 0, "a lane keeps its columns");
   float* rows = reinterpret_cast<float*>(lin_smem) + wave * (32 * PITCH);
   const int c = (lane % LANES) * 4, n = n0 + wn + c, r0 = lane / LANES;
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void linear_row_n_kernel(LinTileArg
     uintx4 wv[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) wv[u] = *reinterpret_cast<const uintx4*>(w + (long long)(k0 + u) * p.ldb);
-    uintx4 xv[MR][8 / EPC];   // packed: eight rows of fp32 would not fit the registers
+    uintx4 xv[MR][8 / EPC];   // packed, to spare registers
 #pragma unroll
     for (int m = 0; m < MR; ++m)
 #pragma unroll
@@ -510,14 +510,14 @@ const LinLaunch& lin_launch_bf16();
 const LinLaunch& lin_launch_f16();
 
 // The variants of the product kernel: tile, waves over it, stages in LDS, 128-byte pieces of k per stage.
-enum LinVariant { LIN_REGS = 0, LIN_64 = 1, LIN_128 = 2, LIN_256 = 3, LIN_ROWS = 4 };
-struct LinTile { int t, wgm, wgn, stages, subs; };
-constexpr LinTile kLinTiles[] = {{128, 2, 2, 1, 1}, {64, 2, 2, 4, 1}, {128, 2, 4, 2, 2}, {256, 2, 4, 2, 1}};
+enum LinVariant { LIN_REGS = 0, LIN_64 = 1, LIN_128 = 2, LIN_256 = 3, LIN_32 = 4, LIN_ROWS = 5 };
+struct LinTile { int tm, tn, wgm, wgn, stages, subs; };
+constexpr LinTile kLinTiles[] = {{128, 128, 2, 2, 1, 1}, {64, 64, 2, 2, 4, 1}, {128, 128, 2, 4, 2, 2}, {256, 256, 2, 4, 2, 1}, {32, 64, 1, 4, 4, 1}};
 
 template <MmKind KIND, bool KCA, bool KCB, int V>
 struct LinLoopOf {
   static constexpr LinTile T = kLinTiles[V];
-  using type = MmDirect<KIND, KCA, KCB, T.t, T.t, T.wgm, T.wgn, true, T.stages, T.subs>;
+  using type = MmDirect<KIND, KCA, KCB, T.tm, T.tn, T.wgm, T.wgn, true, T.stages, T.subs>;
 };
 template <MmKind KIND, bool KCA, bool KCB>
 struct LinLoopOf<KIND, KCA, KCB, LIN_REGS> {
@@ -528,7 +528,7 @@ void lin_tile_launch_as(const LinTileArgs& a, hipStream_t stream) {
   constexpr LinTile T = kLinTiles[V];
   constexpr int WAVES = T.wgm * T.wgn;
   using Loop = typename LinLoopOf<KIND, KCA, KCB, V>::type;
-  launch("linear", linear_tile_kernel<KIND, Loop, T.t, T.t, T.wgm, T.wgn>, dim3((unsigned)((a.total + 7) / 8 * 8)), dim3(64 * WAVES), lin_lds<Loop, WAVES>(),
+  launch("linear", linear_tile_kernel<KIND, Loop, T.tm, T.tn, T.wgm, T.wgn>, dim3((unsigned)((a.total + 7) / 8 * 8)), dim3(64 * WAVES), lin_lds<Loop, WAVES>(),
          stream, a);
 }
 // columns of a workgroup of the few-rows kernel over W [K,N], by lanes side by side
@@ -553,11 +553,12 @@ void lin_row_launch_as(const LinTileArgs& a, hipStream_t stream) {
 }
 template <MmKind KIND, bool KCB>
 void lin_row_launch(const LinTileArgs& a, hipStream_t stream) {
-  if (a.p.M <= 1) lin_row_launch_as<KIND, 1, KCB>(a, stream);
-  else if (a.p.M <= 2) lin_row_launch_as<KIND, 2, KCB>(a, stream);
-  else if (a.p.M <= 4) lin_row_launch_as<KIND, 4, KCB>(a, stream);
-  else if constexpr (KIND == MM_F32) lin_row_launch_as<KIND, 8, KCB>(a, stream);
-  else throw std::runtime_error("linear: too many rows");
+  if (a.p.M <= 1) return lin_row_launch_as<KIND, 1, KCB>(a, stream);
+  if constexpr (KIND == MM_F32 || KCB)
+    if (a.p.M <= 2) return lin_row_launch_as<KIND, 2, KCB>(a, stream);
+  if constexpr (KIND == MM_F32)
+    if (a.p.M <= 4) return lin_row_launch_as<KIND, 4, KCB>(a, stream);
+  throw std::runtime_error("linear: too many rows");
 }
 template <MmKind KIND, bool KCA, bool KCB>
 void lin_tile_launch(const LinTileArgs& a, int variant, hipStream_t stream) {
@@ -566,6 +567,9 @@ void lin_tile_launch(const LinTileArgs& a, int variant, hipStream_t stream) {
     case LIN_64: return lin_tile_launch_as<KIND, KCA, KCB, LIN_64>(a, stream);
     case LIN_128: return lin_tile_launch_as<KIND, KCA, KCB, LIN_128>(a, stream);
     case LIN_256: return lin_tile_launch_as<KIND, KCA, KCB, LIN_256>(a, stream);
+    case LIN_32:
+      if constexpr (KCA) return lin_tile_launch_as<KIND, KCA, KCB, LIN_32>(a, stream);
+      [[fallthrough]];
     case LIN_ROWS:
       if constexpr (KCA) return lin_row_launch<KIND, KCB>(a, stream);
       [[fallthrough]];
@@ -589,7 +593,10 @@ LinLaunch lin_make_launch() {
     launch("linear_join", linear_join_kernel<KIND>, dim3((unsigned)(blocks > 4096 ? 4096 : blocks)), dim3(256), 0, s, a);
   };
   l.dz = [](const LinDzArgs& a, dim3 grid, hipStream_t s) { launch("linear_dz", linear_dz_kernel<KIND>, grid, dim3(256), 0, s, a); };
-  l.pad = [](const LinPadArgs& a, hipStream_t s) { launch("linear_pad", linear_pad_kernel<KIND>, dim3(1024, 2), dim3(256), 0, s, a); };
+  l.pad = [](const LinPadArgs& a, hipStream_t s) {
+    const int rows = a.rows[0] > a.rows[1] ? a.rows[0] : a.rows[1];
+    launch("linear_pad", linear_pad_kernel<KIND>, dim3((unsigned)(rows > 8192 ? 2048 : ceil_div(rows, 4)), 2), dim3(256), 0, s, a);
+  };
   l.colsum = [](const LinColSumArgs& a, hipStream_t s) {
     launch("linear_colsum", linear_colsum_kernel<KIND>, dim3((unsigned)ceil_div(a.N, 64)), dim3(256), 0, s, a);
   };

@@ -9,6 +9,7 @@ instead of silently falling back to PyTorch ops.
 from __future__ import annotations
 
 import functools
+import itertools
 import math
 from dataclasses import dataclass
 from typing import Dict, Optional
@@ -1369,14 +1370,15 @@ def muon_step(p, g, m, v, hyper, tables: MuonTables, *, nesterov: bool, steps: i
 def linear_workspace(m: int, n: int, k: int, dtype=torch.float32, trans_w: bool = False) -> int:
     """Bytes of workspace that linear() may need for x [m,k] and n outputs, whatever the tensors' strides."""
     ldw = k if trans_w else n
-    return max(hip().linear_workspace(_KINDS[dtype], m, n, k, trans_w, 0, at, k, at, ldw, 0, 0, 0, 0, n, 0, 0) for at in (0, 1))   # aligned or not
+    return max(hip().linear_workspace(_KINDS[dtype], m, n, k, trans_w, 0, x, k, w, ldw, 0, 0, 0, 0, n, 0, 0)
+               for x, w in itertools.product((0, 1), repeat=2))   # addresses, aligned or not
 
 
 def linear_bwd_workspace(m: int, n: int, k: int, dtype=torch.float32, trans_w: bool = False, activation: str = "none") -> int:
     """Bytes of workspace that linear_bwd() may need for dy [m,n] and x [m,k] with all three gradients."""
     ldw = k if trans_w else n
-    return max(hip().linear_bwd_workspace(_KINDS[dtype], m, n, k, trans_w, ACTIVATIONS[activation], False, at, n, 0, n, at, k, at, ldw, 1, k, 1, ldw, 1)
-               for at in (0, 1))
+    return max(hip().linear_bwd_workspace(_KINDS[dtype], m, n, k, trans_w, ACTIVATIONS[activation], False, dy, n, 0, n, x, k, w, ldw, 1, k, 1, ldw, 1)
+               for dy, x, w in itertools.product((0, 1), repeat=3))
 
 
 def col_sum(x2d, out, relu_of=None, masked=None):

@@ -110,6 +110,35 @@ def test_linear_large(m, k, n, trans_w, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("m,k,n", [(2, 1785, 283), (3, 973, 628), (5, 1024, 264), (9, 712, 3720), (23, 1000, 136), (31, 65, 260), (40, 8128, 264),
+                                   (250, 2216, 304), (2, (1 << 20) + 5, 9), (70, (1 << 20) + 1, 3)])
+def test_linear_few_rows_and_long_lines(m, k, n, trans_w, dtype):
+    """32-row tiles, k in many parts, copies for few rows, and lines too long for a copy; forward and gradients."""
+    x, w, bias, res = make(m, k, n, dtype, trans_w, seed=14)
+    pre = torch.empty(m, n, device="cuda", dtype=dtype)
+    y = nv.linear(x, w, bias, activation="silu", residual=res, trans_w=trans_w, pre=pre)
+    check_forward(x, w, bias, res, "silu", trans_w, y, pre)
+    check_backward(res, x, w, pre, "silu", trans_w, *nv.linear_bwd(res, x, w, pre=pre, activation="silu", trans_w=trans_w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(3, 1000, 64), (20, 4096, 40), (70, 72, 136), (2, (1 << 20) + 8, 16), (2, 1 << 20, 24)])
+def test_linear_workspace_covers_every_alignment(m, k, n):
+    for trans_w in (False, True):
+        for shift_x in (0, 1):
+            for shift_w in (0, 1):
+                x, _, bias, dy = make(m, k, n, torch.bfloat16, trans_w, shift=shift_x)
+                _, w, _, _ = make(m, k, n, torch.bfloat16, trans_w, shift=shift_w)
+                ws = torch.empty(nv.linear_workspace(m, n, k, torch.bfloat16, trans_w), device="cuda", dtype=torch.uint8)
+                assert torch.equal(nv.linear(x, w, bias, trans_w=trans_w, workspace=ws), nv.linear(x, w, bias, trans_w=trans_w))
+                ws = torch.empty(nv.linear_bwd_workspace(m, n, k, torch.bfloat16, trans_w), device="cuda", dtype=torch.uint8)
+                for a, b in zip(nv.linear_bwd(dy, x, w, trans_w=trans_w, workspace=ws), nv.linear_bwd(dy, x, w, trans_w=trans_w)):
+                    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("ld", [(1 << 22) - 8, (1 << 24) + 8, (1 << 22) + 3])
 def test_linear_rows_far_apart(ld):
     """Rows whose addresses pass 2^31 and 2^32 bytes, read and written, below and above the stride that one 32-bit offset covers."""
