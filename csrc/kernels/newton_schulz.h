@@ -38,8 +38,9 @@ __host__ __device__ inline long long ns_floats(const NsMat& m) { return 2 * kNsN
 // Fills in everything but the offsets.
 void ns_shape(NsMat& m, int rows, int cols);
 
-// Matrices whose steps all run in one workgroup.
-inline bool ns_small(const NsMat& m) { return m.r <= 32 ? m.c <= 1024 : m.r <= 64 && m.c <= 768; }
+// Matrices whose steps all run in one workgroup (us that way / by tiles: 10 x 1039 36 / 90, 16 x 2048 43 / 92; what does not fit its registers
+// takes 95 - 105 by tiles: 32 x 2048, 64 x 1024).
+inline bool ns_small(const NsMat& m) { return m.r <= 16 ? m.c <= 2048 : m.r <= 32 ? m.c <= 1024 : m.r <= 64 && m.c <= 768; }
 
 // A work item. Split X X^T: kn blocks of 32 columns of X from k0 on, its sums into slot `slot`; joining it: kn slots from `slot` on.
 struct NsItem { int mat, tile, k0, kn, slot, pad; };

@@ -616,7 +616,8 @@ __global__ __launch_bounds__(64 * kSmallWaves) void ns_small_kernel(NsSmallArgs 
 #define NS_SMALL(RT, NB) ns_small_run<RT, NB>(a.d, m, a.co, a.steps, ns_smem)
   if (m.r <= 16) {
     if (nb == 1) NS_SMALL(1, 1);
-    else NS_SMALL(1, 4);
+    else if (nb <= 4) NS_SMALL(1, 4);
+    else NS_SMALL(1, 8);
   } else if (m.r <= 32) {
     if (nb <= 2) NS_SMALL(2, 2);
     else NS_SMALL(2, 4);

@@ -88,6 +88,14 @@ def test_newton_schulz_large(m, n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(1, 2048), (9, 1486), (2000, 9), (16, 2048), (1025, 16), (16, 2049), (17, 1100)])
+def test_newton_schulz_few_long_rows(m, n, dtype):
+    g = gradient(m, n, seed=5, scale=1.0).to(dtype).cuda()
+    check(nv.newton_schulz(g), g)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("batch", [1, 2, 6, 40])
 @pytest.mark.parametrize("m,n", [(576, 64), (48, 40), (20, 200)])
 def test_newton_schulz_batches(m, n, batch):
