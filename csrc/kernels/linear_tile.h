@@ -143,6 +143,14 @@ __device__ __forceinline__ void lin_finish(const MmProduct& p, int vec, int m, i
   lin_finish<KIND>(p, vec, m, n, v, lin_bias<KIND>(p, vec, n), lin_read<KIND>(p, vec, m, n));
 }
 
+// Lanes of a wave that hand each other values through LDS: a wave's accesses of LDS happen in order, so all it takes is that the compiler
+// keeps every access on its side of this point, and the lanes together at it. No instruction.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 template <int NJ>
 struct LinEpilogue { static constexpr int PITCH = NJ * 16 + 4; };   // floats; the 16 bytes spread a column over the banks
 template <class Loop, int WAVES>
@@ -174,7 +182,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tile_kernel(LinTileArgs
 
   // The sums leave through LDS, 32 rows of a wave's tile at a time: a loop over whole rows with 16 lanes to a row, so the
   // tensors are read and written 64 columns at once and the epilogue's code exists once. Each wave has its own rows: no barrier.
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, l15 = lane & 15;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));   // what follows from it is computed here, not kept in registers over the product
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), q = lane >> 4, l15 = lane & 15;
   const int wm = (wave / WGN) * (BM / WGM), wn = (wave % WGN) * (BN / WGN);
   constexpr int PITCH = LinEpilogue<NJ>::PITCH, LANES = NJ * 4, RSTEP = 64 / LANES, U = RSTEP > 8 ? 32 / RSTEP : 4;   // lanes to a row, rows at once, reads ahead
   static_assert(64 % LANES == 0 && 32 % (RSTEP * U) == 0, "a lane keeps its columns");
@@ -190,26 +200,29 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tile_kernel(LinTileArgs
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) *reinterpret_cast<floatx4*>(rows + (i * 16 + l15) * PITCH + j * 16 + 4 * q) = acc[i0 + i][j];
-    if (n >= p.N) continue;
+    wave_lds_fence();
+    if (n < p.N) {   // the lanes without a column wait at the fence below
 #pragma unroll 1
-    for (int r = r0; r < 32; r += RSTEP * U) {
-      if (a.splits > 1) {
+      for (int r = r0; r < 32; r += RSTEP * U) {
+        if (a.splits > 1) {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (mb + r + u * RSTEP < p.M)   // N4 covers the last n
+              *reinterpret_cast<floatx4*>(a.partial + ((long long)split * p.M + mb + r + u * RSTEP) * a.N4 + n) =
+                  *reinterpret_cast<const floatx4*>(rows + (r + u * RSTEP) * PITCH + c);
+          continue;
+        }
+        LinRead<KIND> rd[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (mb + r + u * RSTEP < p.M)   // N4 covers the last n
-            *reinterpret_cast<floatx4*>(a.partial + ((long long)split * p.M + mb + r + u * RSTEP) * a.N4 + n) =
-                *reinterpret_cast<const floatx4*>(rows + (r + u * RSTEP) * PITCH + c);
-        continue;
+          if (mb + r + u * RSTEP < p.M) rd[u] = lin_read<KIND>(p, a.vec, mb + r + u * RSTEP, n);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (mb + r + u * RSTEP < p.M)
+            lin_finish<KIND>(p, a.vec, mb + r + u * RSTEP, n, *reinterpret_cast<const floatx4*>(rows + (r + u * RSTEP) * PITCH + c), bias, rd[u]);
       }
-      LinRead<KIND> rd[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (mb + r + u * RSTEP < p.M) rd[u] = lin_read<KIND>(p, a.vec, mb + r + u * RSTEP, n);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (mb + r + u * RSTEP < p.M)
-          lin_finish<KIND>(p, a.vec, mb + r + u * RSTEP, n, *reinterpret_cast<const floatx4*>(rows + (r + u * RSTEP) * PITCH + c), bias, rd[u]);
     }
+    wave_lds_fence();
   }
 }
 
