@@ -21,6 +21,7 @@ struct MmProduct {
   void* pre;                // nullable, [M,N]: receives the value before the activation
   long long ldp;
   int act;
+  float scale;              // a power of two: C = act(scale A B + bias) + res
   int accumulate;           // C += result
 };
 size_t mm_product_workspace(const MmProduct& p);

@@ -197,12 +197,14 @@ MmProduct forward_of(const LinearArgs& a) {
   p.c = a.y; p.ldc = a.ldy;
   p.bias = a.bias; p.res = a.res; p.ldr = a.ldr; p.pre = a.pre; p.ldp = a.ldp;
   p.act = a.act;
+  p.scale = 1.f;
   return p;
 }
 struct BwdPlan {
   MmProduct dx, dw;
   int rows, blocks;
   long long N4, lddz;
+  float dz_scale;
   size_t dz_bytes, part_bytes, prod_bytes;
 };
 BwdPlan bwd_plan(const LinearBwdArgs& a, void* dz) {
@@ -212,6 +214,10 @@ BwdPlan bwd_plan(const LinearBwdArgs& a, void* dz) {
   const bool own_dz = a.act != ACT_NONE && (a.dx || a.dw);
   b.N4 = ((long long)a.N + 3) / 4 * 4;
   b.lddz = ((long long)a.N + 7) / 8 * 8;
+  // Slopes reach 1.13 (gelu, gelu_tanh) and 1.10 (silu): times an fp16 dy near 65504 they leave the type's range, where the sums of dx and dw need
+  // not. There dz is kept halved and the products doubled, exactly but below 2^-13, where a value keeps one bit less (multiples of 2^-23).
+  b.dz_scale = own_dz && a.kind == MM_F16 && a.act != ACT_RELU ? 0.5f : 1.f;
+  b.dx.scale = b.dw.scale = 1.f / b.dz_scale;
   b.rows = dz_rows(a.M, a.N);
   b.blocks = ceil_div(a.M, b.rows);
   b.dz_bytes = own_dz ? round_up((size_t)a.M * b.lddz * elem_bytes(a.kind)) : 0;
@@ -261,7 +267,7 @@ void linear_bwd(const LinearBwdArgs& a, void* ws, size_t ws_bytes, hipStream_t s
       d.dy = a.dy; d.lddy = a.lddy; d.pre = a.pre; d.ldp = a.ldp;
       d.dz = b.dz_bytes ? at : nullptr; d.lddz = b.lddz;
       d.part = a.db ? part : nullptr; d.N4 = b.N4;
-      d.M = a.M; d.N = a.N; d.act = a.act; d.rows_per_block = b.rows;
+      d.M = a.M; d.N = a.N; d.act = a.act; d.rows_per_block = b.rows; d.dz_scale = b.dz_scale;
       const int v4 = 4 * elem_bytes(a.kind);
       d.vec = !(a.N & 3) && !(a.lddy & 3) && aligned_to(a.dy, v4) && (a.act == ACT_NONE || (!(a.ldp & 3) && aligned_to(a.pre, v4)));
       f.dz(d, dim3((unsigned)ceil_div(a.N, 256), (unsigned)b.blocks), stream);

@@ -124,7 +124,7 @@ __device__ __forceinline__ LinRead<KIND> lin_read(const MmProduct& p, int vec, i
 template <MmKind KIND>
 __device__ __forceinline__ void lin_finish(const MmProduct& p, int vec, int m, int n, floatx4 v, const floatx4& bias, const LinRead<KIND>& r) {
   const int have = p.N - n;
-  v += bias;
+  v = v * p.scale + bias;
   if (p.pre) lin_store4<KIND>(p.pre, (long long)m * p.ldp + n, vec, have, v);
   if (p.act != ACT_NONE) {
 #pragma unroll
@@ -405,6 +405,7 @@ struct LinDzArgs {
   float* part;                 // [row blocks][N4], null: no sums
   long long N4;
   int M, N, act, rows_per_block;
+  float dz_scale;              // dz is stored times this
   int vec;
   AbortRef abort;
 };
@@ -435,7 +436,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinDzArgs a) {
           for (int i = 0; i < 4; ++i)
             if (i < have) v[u][i] *= lin_act_grad<KIND>(a.act, z[u][i]);
         }
-        if (a.dz) lin_store4<KIND>(a.dz, (long long)m * a.lddz + n, 1, 4, v[u]);   // zeros past N
+        if (a.dz) lin_store4<KIND>(a.dz, (long long)m * a.lddz + n, 1, 4, v[u] * a.dz_scale);   // zeros past N
         s += v[u];
       }
     }

@@ -1177,7 +1177,8 @@ def linear_bwd(dy, x, w, *, pre=None, activation: str = "none", trans_w: bool = 
     dy [M,N]; pre [M,N] as linear stored it (not needed for activation "none"). The residual's gradient is dy.
     dx / dw / db: True allocates the output, a tensor receives it, False or None leaves it out. accumulate=True adds
     to the dw and db that are given (dx is always written). dz is rounded to the tensors' type before the two
-    products (exact for none and relu); db sums the unrounded values. Returns (dx, dw, db), None where left out."""
+    products (exact for none and relu; fp16: never past its range, and to multiples of 2^-23 near zero); db sums the
+    unrounded values. Returns (dx, dw, db), None where left out."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"linear_bwd: unknown activation {activation!r}")
