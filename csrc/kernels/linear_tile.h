@@ -50,26 +50,27 @@ __device__ __forceinline__ float lin_act(int act, float z) {
     default: return z;
   }
 }
+// dy act'(z). ReLU selects: whatever arrives at a unit that is off stays there.
 template <MmKind KIND>
-__device__ __forceinline__ float lin_act_grad(int act, float z) {
+__device__ __forceinline__ float lin_act_bwd(int act, float dy, float z) {
   float gauss;
   // Every slope has reached its limit long before: no z^2 that overflows and no infinity times zero. NaN stays.
   z = z > 1e4f ? 1e4f : z < -1e4f ? -1e4f : z;
   switch (act) {
-    case ACT_RELU: return z > 0.f ? 1.f : 0.f;
+    case ACT_RELU: return z > 0.f ? dy : z <= 0.f ? 0.f : z;
     case ACT_GELU: {
       const float phi = lin_phi<KIND>(z, gauss);
-      return phi + z * gauss * 0.39894228040143268f;
+      return dy * (phi + z * gauss * 0.39894228040143268f);
     }
     case ACT_GELU_TANH: {
       const float q = lin_logistic<KIND>(1.5957691216057308f * (z + 0.044715f * z * z * z));
-      return q + z * q * (1.f - q) * (1.5957691216057308f * (1.f + 0.134145f * z * z));
+      return dy * (q + z * q * (1.f - q) * (1.5957691216057308f * (1.f + 0.134145f * z * z)));
     }
     case ACT_SILU: {
       const float q = lin_logistic<KIND>(z);
-      return q * (1.f + z * (1.f - q));
+      return dy * (q * (1.f + z * (1.f - q)));
     }
-    default: return 1.f;
+    default: return dy;
   }
 }
 
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinDzArgs a) {
         if (a.act != ACT_NONE) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (i < have) v[u][i] *= lin_act_grad<KIND>(a.act, z[u][i]);
+            if (i < have) v[u][i] = lin_act_bwd<KIND>(a.act, v[u][i], z[u][i]);
         }
         if (a.dz) lin_store4<KIND>(a.dz, (long long)m * a.lddz + n, 1, 4, v[u] * a.dz_scale);   // zeros past N
         s += v[u];

@@ -1175,6 +1175,7 @@ def linear_bwd(dy, x, w, *, pre=None, activation: str = "none", trans_w: bool = 
     """Gradients of linear(): dz = dy act'(pre); dx = dz W^T, dw = x^T dz (laid out like w), db = column sums of dz.
 
     dy [M,N]; pre [M,N] as linear stored it (not needed for activation "none"). The residual's gradient is dy.
+    relu selects: dz is 0 where pre <= 0 whatever dy holds there, and NaN where pre is.
     dx / dw / db: True allocates the output, a tensor receives it, False or None leaves it out. accumulate=True adds
     to the dw and db that are given (dx is always written). dz is rounded to the tensors' type before the two
     products (exact for none and relu; fp16: never past its range, and to multiples of 2^-23 near zero); db sums the

@@ -47,3 +47,26 @@ def test_fp16_gradients_near_the_smallest_numbers(act):
     close(dx, dz @ w64.t(), off @ w64.abs().t() + (n + 4) * U * (size @ w64.abs().t()), torch.float16, "dx")
     close(dw, x64.t() @ dz, x64.abs().t() @ off + (m + 4) * U * (x64.abs().t() @ size), torch.float16, "dw")
     close(db, dz.sum(0), (dy.double().abs() * 16 * U).sum(0) + (m + 4) * U * dz.abs().sum(0), torch.float16, "db")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(3, 8, 5), (40, 24, 56)])
+def test_relu_gradient_of_units_that_are_off(m, k, n, dtype):
+    """An infinite or NaN dy at a unit that ReLU shut off leaves no trace; a NaN pre-activation stays one."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    dy, pre, x, w = ((torch.randn(*s, device="cuda", generator=g)).to(dtype) for s in ((m, n), (m, n), (m, k), (k, n)))
+    pre[0, :3] = torch.tensor([-1.0, 0.0, -0.0])
+    pre[1, 0], pre[2, 2] = float("-inf"), -3.0
+    clean = dy.clone()
+    clean[pre <= 0] = 0
+    want = nv.linear_bwd(clean, x, w, pre=pre, activation="relu")
+    dy[0, :3] = torch.tensor([float("inf"), float("-inf"), float("nan")])
+    dy[1, 0] = float("nan")
+    dy[2, 2] = float("inf")
+    for a, b in zip(nv.linear_bwd(dy, x, w, pre=pre, activation="relu"), want):
+        assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+    pre[2, 1] = float("nan")
+    dx, dw, db = nv.linear_bwd(dy, x, w, pre=pre, activation="relu")
+    rows, cols = torch.arange(m, device="cuda") == 2, torch.arange(n, device="cuda") == 1
+    assert torch.equal(dx.isnan(), rows[:, None].expand(m, k)) and torch.equal(dw.isnan(), cols.expand(k, n)) and torch.equal(db.isnan(), cols)
