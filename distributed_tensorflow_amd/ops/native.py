@@ -1364,6 +1364,8 @@ def muon_step(p, g, m, v, hyper, tables: MuonTables, *, nesterov: bool, steps: i
         raise ValueError("muon_step: size mismatch")
     if any(t.get_device() != torch.cuda.current_device() for t in (p, g, m, v, hyper, tables.workspace)):
         raise ValueError("muon_step: the buffers are not on the current device")
+    if not eps > 0:
+        raise ValueError("muon_step: eps must be positive")
     flat, growth = _ns_steps(_ns_key(coeffs), steps)
     hip().muon_step(dict(p=_chk(p, "p"), g=_chk(g, "g"), m=_chk(m, "m"), v=_chk(v, "v"), hyper=_chk(hyper, "hyper"), nesterov=int(nesterov),
                          coeffs=flat, growth=growth, eps=float(eps), **tables.launch_args()), stream())

@@ -113,6 +113,8 @@ class FlatMuon(_FlatOptimizer):
                  ns_coeffs=ref.NS_COEFFS, ns_eps: float = 1e-7, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
                  matrices: Optional[Iterable[str]] = None):
         super().__init__(arena)
+        if not ns_eps > 0:
+            raise ValueError("FlatMuon: ns_eps must be positive")   # a matrix without a gradient would be 0 / 0
         self.momentum, self.nesterov, self.weight_decay = momentum, nesterov, weight_decay
         self.ns_steps, self.ns_coeffs, self.ns_eps = ns_steps, ns_coeffs, ns_eps
         self.beta1, self.beta2, self.eps = beta1, beta2, eps
