@@ -1355,6 +1355,11 @@ class MuonTables:
         return d
 
 
+def check_current_device(what: str, *tensors: torch.Tensor) -> None:
+    if any(t.get_device() != torch.cuda.current_device() for t in tensors):
+        raise ValueError(f"{what}: the buffers are not on the current device")
+
+
 def muon_step(p, g, m, v, hyper, tables: MuonTables, *, nesterov: bool, steps: int, coeffs=NS_COEFFS, eps: float = 1e-7):
     """One orthogonalised-momentum step over a flat buffer (csrc/kernels/newton_schulz.hip). hyper: lr, momentum,
     grad_scale, 1 - lr * weight_decay, then the vectors' Adam step size, 1 - beta1, 1 - beta2 and epsilon."""
@@ -1362,8 +1367,7 @@ def muon_step(p, g, m, v, hyper, tables: MuonTables, *, nesterov: bool, steps: i
     n = p.numel()
     if g.numel() != n or m.numel() != n or v.numel() != n or hyper.numel() < HYPER_SLOTS:
         raise ValueError("muon_step: size mismatch")
-    if any(t.get_device() != torch.cuda.current_device() for t in (p, g, m, v, hyper, tables.workspace)):
-        raise ValueError("muon_step: the buffers are not on the current device")
+    check_current_device("muon_step", p, g, m, v, hyper, tables.workspace)
     if not eps > 0:
         raise ValueError("muon_step: eps must be positive")
     flat, growth = _ns_steps(_ns_key(coeffs), steps)

@@ -142,6 +142,7 @@ class FlatMuon(_FlatOptimizer):
         a, t = self.arena, self.steps + 1
         lr_t = (lr if vector_lr is None else vector_lr) * math.sqrt(1.0 - self.beta2 ** t) / (1.0 - self.beta1 ** t)
         if self._gpu:
+            self._nv.check_current_device("FlatMuon", a.params, self._hyper, self._tables.workspace)   # the scalars are a launch already
             self._nv.set_scalars(self._hyper, (lr, self.momentum, grad_scale, 1.0 - lr * self.weight_decay, lr_t, 1.0 - self.beta1,
                                                1.0 - self.beta2, self.eps))
             self._nv.muon_step(a.params, a.grads, a.slots["m"], a.slots["v"], self._hyper, self._tables, nesterov=self.nesterov,
