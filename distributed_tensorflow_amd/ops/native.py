@@ -1109,14 +1109,17 @@ def _check_apart(what: str, written, read, in_place=()) -> None:
                 raise ValueError(f"{what}: an output overlaps another tensor of the call")
 
 
-def _workspace(what: str, need: int, workspace: Optional[torch.Tensor], device) -> tuple:
-    """(tensor, address, bytes): the caller's workspace, or one from torch's allocator for the current stream."""
+def _workspace(what: str, need: int, workspace: Optional[torch.Tensor], device, tensors=()) -> tuple:
+    """(tensor, address, bytes): the caller's workspace, which `tensors` may not reach into, or one from torch's allocator for the
+    current stream."""
     if workspace is not None:
         if workspace.device != device or not workspace.is_contiguous() or workspace.data_ptr() % 16:
             raise ValueError(f"{what}: the workspace must be contiguous, 16-byte aligned and on the tensors' device")
         have = workspace.numel() * workspace.element_size()
         if have < need:
             raise ValueError(f"{what}: the workspace has {have} bytes, {need} are needed")
+        if any(t is not None and _overlap(workspace, t) for t in tensors):
+            raise ValueError(f"{what}: the workspace overlaps a tensor of the call")
         return workspace, workspace.data_ptr(), have
     if need == 0:
         return None, 0, 0
@@ -1163,7 +1166,7 @@ def linear(x, w, bias=None, *, activation: str = "none", residual=None, trans_w:
     args = (_KINDS[x.dtype], m, n, k, trans_w, act, px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pp, ldp)
     need = _hip.linear_workspace(*args)
     if need or workspace is not None:
-        ws, addr, have = _workspace("linear", need, workspace, x.device)
+        ws, addr, have = _workspace("linear", need, workspace, x.device, (x, w, bias, residual, out, pre))
         _hip.linear(*args, addr, have, _raw_stream(dev))
     else:
         _hip.linear(*args, 0, 0, _raw_stream(dev))
@@ -1215,7 +1218,8 @@ def linear_bwd(dy, x, w, *, pre=None, activation: str = "none", trans_w: bool = 
         pdb = db.data_ptr()
     dev = _check_device(dy, "linear_bwd")
     args = (_KINDS[dy.dtype], m, n, k, trans_w, act, accumulate, pdy, lddy, pp, ldp, px, ldx, pw, ldw, pdx, lddx, pdw, lddw, pdb)
-    ws, addr, have = _workspace("linear_bwd", _hip.linear_bwd_workspace(*args), workspace, dy.device)
+    need = _hip.linear_bwd_workspace(*args)
+    ws, addr, have = _workspace("linear_bwd", need, workspace, dy.device, (dy, x, w, pre if act else None, dx, dw, db))
     _hip.linear_bwd(*args, addr, have, _raw_stream(dev))
     return dx, dw, db
 
@@ -1289,7 +1293,8 @@ def newton_schulz(g, *, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out
         return out
     batch = g.shape[0] if g.dim() == 3 else 1
     kind = _KINDS[g.dtype]
-    ws, addr, have = _workspace("newton_schulz", _hip.newton_schulz_workspace(kind, batch, rows, cols), workspace, g.device)
+    need = _hip.newton_schulz_workspace(kind, batch, rows, cols)
+    ws, addr, have = _workspace("newton_schulz", need, workspace, g.device, (g, out))
     _hip.newton_schulz(kind, batch, rows, cols, *pg, *po, eps, flat, growth, addr, have, _raw_stream(dev))
     return out
 
