@@ -1074,6 +1074,11 @@ def _check_device(t: torch.Tensor, what: str) -> int:
     return dev
 
 
+def _check_no_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what}: autograd does not see this call, and a tensor requires a gradient: call it under torch.no_grad(), or detach")
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the current stream's handle without a Stream object around it
 
 
@@ -1136,7 +1141,9 @@ def linear(x, w, bias=None, *, activation: str = "none", residual=None, trans_w:
     type, float32, bfloat16 or float16; sums are fp32 (float32 products run on the exact fp32 matrix pipe) and every
     output is rounded once. Matrices may be row-strided views. activation: none, relu, gelu (erf), gelu_tanh, silu.
     pre [M,N] receives x W + bias for linear_bwd. out may be `residual` itself, otherwise outputs overlap nothing.
-    workspace: linear_workspace() bytes; a call recorded into a step program has to bring its own. Not differentiated by autograd."""
+    workspace: linear_workspace() bytes; a call recorded into a step program has to bring its own. Not differentiated by autograd: tensors
+    that require gradients are taken under torch.no_grad() only."""
+    _check_no_grad("linear", x, w, bias, residual)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"linear: unknown activation {activation!r}")
@@ -1183,6 +1190,7 @@ def linear_bwd(dy, x, w, *, pre=None, activation: str = "none", trans_w: bool = 
     to the dw and db that are given (dx is always written). dz is rounded to the tensors' type before the two
     products (exact for none and relu; fp16: never past its range, and to multiples of 2^-23 near zero); db sums the
     unrounded values. Returns (dx, dw, db), None where left out."""
+    _check_no_grad("linear_bwd", dy, x, w, pre)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"linear_bwd: unknown activation {activation!r}")
@@ -1268,6 +1276,7 @@ def newton_schulz(g, *, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out
     type, since five steps amplify an early rounding error up to 485-fold. Rows may be strided. coeffs: (a, b, c), or
     a triple for every step; sequences whose iterates would leave the pairs' range are refused. out may be g itself.
     workspace: newton_schulz_workspace() bytes; a call recorded into a step program has to bring its own."""
+    _check_no_grad("newton_schulz", g)
     if g.dim() not in (2, 3):
         raise ValueError("newton_schulz: a matrix or a batch of matrices")
     if not eps > 0:
