@@ -61,13 +61,17 @@ __device__ __forceinline__ void mm_mfma_all(const Frag& x, const Frag& y, floatx
 
 // 16 bytes per lane from memory to LDS at lds + 16 lane, past the registers; done when vmcnt says so. Written in asm
 // because the compiler, which cannot tell the two stages of a double buffer apart, would wait for every such load
-// before the next read of LDS. There is no output register; M0 is written in the same block and has no other use here.
+// before the next read of LDS. There is no output register. M0 is written in the same block and named as lost: the compiler, which reserves the
+// register for instructions of its own and sets it right in front of them, remarks on that (inline-asm).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void lds_load16(const char* base, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void lds_load16_any(const char* p, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(p) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(p) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // All but the last PENDING loads of this wave have landed, every read of LDS has returned, and all waves are here.
 template <int PENDING>
 __device__ __forceinline__ void lds_stage_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(PENDING) : "memory"); }

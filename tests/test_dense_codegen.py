@@ -61,3 +61,15 @@ def test_lanes_that_exchange_sums_through_lds_are_kept_in_step(kernels):
                 events += "B"
         assert "S" in events and "L" in events, name
         assert "SL" not in events and "LS" not in events, f"{name}: {events}"
+
+
+@needs_hipcc
+def test_asm_that_writes_m0_says_so(kernels):
+    """The compiler uses M0 for instructions of its own: a block that writes it has to be in its list."""
+    seen = 0
+    for name, lines in kernels.items():
+        for line in lines:
+            if " asm " in line and re.search(r"\bm0\b", line.split('"')[1]):
+                seen += 1
+                assert "~{m0}" in line, f"{name}: {line.strip()}"
+    assert seen > 0
