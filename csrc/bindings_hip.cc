@@ -551,7 +551,7 @@ PYBIND11_MODULE(_hip, m) {
     m.def("ns_shape", [](int rows, int cols) {
       NsMat x{};
       ns_shape(x, rows, cols);
-      return py::make_tuple(x.r, x.c, x.rp, x.cp, x.tall, x.parts, x.chunk, x.sx, ns_floats(x), ns_small(x));
+      return py::make_tuple(x.r, x.c, x.rp, x.cp, x.tall, x.parts, x.chunk, ns_floats(x), ns_small(x));
     });
     m.def("ns_splits", [](int rows, int cols, long long tiles) {
       NsMat x{};

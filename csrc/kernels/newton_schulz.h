@@ -26,9 +26,7 @@ struct NsMat {
   int r, c, rp, cp;     // r = min, c = max side; padded
   int tall;             // rows > cols: X = G^T
   int parts, chunk;     // pieces of the norm, elements each
-  float sx;             // X is kept times sx (a power of two that brings typical elements to 1)
   float scale;          // optimizer: W <- decay W - lr scale O
-  int pad;
 };
 __host__ __device__ inline long long ns_x_floats(const NsMat& m) { return (long long)m.rp * m.cp; }
 __host__ __device__ inline long long ns_x(const NsMat& m) { return m.ws + 2 * kNsNormParts + 64; }

@@ -2,8 +2,10 @@
 //
 // Precision: five steps amplify a rounding error in a direction of a small singular value 485-fold. Single bf16 or fp16
 // operands leave errors of 3 - 30 % / 0.4 - 4 % in the result; h + l with 22 bits and the three products hh + hl + lh (mm_tile.h)
-// measures within 10 % of what fp32 products leave (1e-6 - 1e-5 relative, 64x10 to 1024x2048). Everything is scaled by powers
-// of two that keep h in fp16's normal range: X by sx ~ sqrt(r c), so that typical elements of X_0 are about 1, A and P by 2^12.
+// measures what fp32 products leave, in the norm of the whole (1e-6 - 1e-5 relative, 64x10 to 1024x2048). Everything is kept times the largest
+// power of two that fits fp16: X by 2^13, A and P by 2^12. An element keeps its 22 bits down to 2^-16 (X) and 2^-15; below, the pair's smallest step is
+// a floor: 2^-38 and 2^-37 at most. Rows or columns far below the others feel it, and fp32 products would not (64 x 256, one row scaled by 1e-2 / 1e-4 / 1e-6:
+// its relative error 2e-7 / 3e-6 / 3e-4, by fp32 products 3e-7).
 // A matrix whose norm is far below eps starts with tiny X_0; its part below one is carried apart in tau (a power of two per
 // matrix, grown by `growth` per step up to 1), so that the fp16 numbers never see it: X = tau Xs,
 //   Xs <- (tau / tau') (a I + b tau^2 As + c tau^4 As^2) Xs.
@@ -16,7 +18,7 @@
 namespace dtf {
 namespace {
 
-constexpr float kScaleA = 4096.f, kScaleP = 4096.f;   // |A| <= 3.8^2 and |P| <= 14 stay below fp16's 65504
+constexpr float kScaleX = 8192.f, kScaleA = 4096.f, kScaleP = 4096.f;   // |X| <= 3.8, |A| <= 3.8^2 and |P| <= 14 stay below fp16's 65504
 
 struct NsDev {
   NsMat one;                   // table == nullptr: `batch` matrices of this shape
@@ -205,7 +207,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsDev a) {
   // tau: the power of two at or above t, 1 unless the norm is below eps (or is not a number)
   float tau = 1.f;
   if (t < 0.5) tau = t > 1e-37 ? ldexpf(1.f, ilogb(t) + 1) : 1.1754944e-38f;
-  const double inv = (double)m.sx / ((norm + a.eps) * (double)tau);
+  const double inv = (double)kScaleX / ((norm + a.eps) * (double)tau);
   const int bc = m.cp / 32, bi = tile / bc, bj = tile - bi * bc;   // block of X
   if (tile == 0 && threadIdx.x == 0) base[2 * kNsNormParts] = tau;
   const int r0 = (m.tall ? bj : bi) * 32, c0 = (m.tall ? bi : bj) * 32;   // block of G
@@ -338,7 +340,7 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
     float* dst = GRAM ? A : P;
     float ca = 0.f, cb = 0.f, cc;   // value = ca I + cb A + cc acc
     if (GRAM) {
-      cc = kScaleA / (m.sx * m.sx);
+      cc = kScaleA / (kScaleX * kScaleX);
     } else {
       const float tau = tau_at(a.ws[m.ws + 2 * kNsNormParts], a.growth, a.step), next = fminf(1.f, tau * a.growth);
       const float s1 = kScaleP * (tau / next), t2 = tau * tau;
@@ -394,7 +396,7 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
   }
   // The output, in G's orientation: a lane holds four consecutive elements of a row of it.
   const float tau = tau_at(a.ws[m.ws + 2 * kNsNormParts], a.growth, a.step + 1);
-  const float f = 1.f / (kScaleP * m.sx);   // tau apart: their product can leave fp32's normal range
+  const float f = 1.f / (kScaleP * kScaleX);   // tau apart: their product can leave fp32's normal range
   const float lr = a.m ? a.hyper[0] * m.scale : 0.f, decay = a.m ? a.hyper[3] : 0.f;
 #pragma unroll
   for (int i = 0; i < MI; ++i)
@@ -496,7 +498,7 @@ __device__ __forceinline__ void ns_small_run(const NsDev& a, const NsMat& m, con
 #pragma unroll
       for (int w = 0; w < kSmallWaves; ++w) s += *reinterpret_cast<const floatx4*>(parts + w * kSmallPart + e * 16);
       const int k = e >> 6, i = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0, j = k - i * (i + 1) / 2;
-      small_store_sym(A, 16 * i + (e & 15), 16 * j + 4 * ((e >> 4) & 3), s * (kScaleA / (m.sx * m.sx)), i != j);
+      small_store_sym(A, 16 * i + (e & 15), 16 * j + 4 * ((e >> 4) & 3), s * (kScaleA / (kScaleX * kScaleX)), i != j);
     }
     __syncthreads();
     const float next = fminf(1.f, tau * a.growth);
@@ -645,7 +647,7 @@ __global__ __launch_bounds__(256) void ns_out_kernel(NsDev a) {
     }
   }
   __syncthreads();
-  const float f = 1.f / m.sx, tau = a.ws[m.ws + 2 * kNsNormParts];
+  const float f = 1.f / kScaleX, tau = a.ws[m.ws + 2 * kNsNormParts];
   const float lr = a.m ? a.hyper[0] * m.scale : 0.f, decay = a.m ? a.hyper[3] : 0.f;
   const int r0 = (m.tall ? bj : bi) * 32, c0 = (m.tall ? bi : bj) * 32;
 #pragma unroll
@@ -701,9 +703,6 @@ void ns_shape(NsMat& m, int rows, int cols) {
   const long long chunk = (n + kNsNormParts - 1) / kNsNormParts;
   m.chunk = (int)(((chunk < 2048 ? 2048 : chunk) + 63) / 64 * 64);
   m.parts = (int)((n + m.chunk - 1) / m.chunk);
-  float s = 1.f;
-  while (s * s < (float)n && s < 8192.f) s *= 2.f;   // the iterates stay below 3.8: 3.8 * 8192 is inside fp16's range
-  m.sx = s;
 }
 
 namespace {

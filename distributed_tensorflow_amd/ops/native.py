@@ -1318,8 +1318,7 @@ class MuonTables:
     launch and the workspace, on the device. `matrices`: (offset, rows, cols); `vectors`: (offset, elements)."""
 
     MAT = np.dtype([("src", "<i8"), ("out", "<i8"), ("ld", "<i8"), ("out_ld", "<i8"), ("ws", "<i8"), ("rows", "<i4"), ("cols", "<i4"), ("r", "<i4"),
-                    ("c", "<i4"), ("rp", "<i4"), ("cp", "<i4"), ("tall", "<i4"), ("parts", "<i4"), ("chunk", "<i4"), ("sx", "<f4"), ("scale", "<f4"),
-                    ("pad", "<i4")])
+                    ("c", "<i4"), ("rp", "<i4"), ("cp", "<i4"), ("tall", "<i4"), ("parts", "<i4"), ("chunk", "<i4"), ("scale", "<f4")])
 
     def __init__(self, matrices, vectors, device):
         require()
@@ -1328,10 +1327,10 @@ class MuonTables:
         mats = np.zeros(len(matrices), dtype=self.MAT)
         flat, small, out, split, gram, join, sym, apply, floats, tile = [], [], [], [], [], [], [], [], 0, h.MUON_TILE
         shapes = [h.ns_shape(rows, cols) for _, rows, cols in matrices]
-        tiles_of = [0 if s[9] else (lambda t: t * (t + 1) // 2)(-(-s[2] // tile)) for s in shapes]   # of X X^T, lower triangle
+        tiles_of = [0 if s[8] else (lambda t: t * (t + 1) // 2)(-(-s[2] // tile)) for s in shapes]   # of X X^T, lower triangle
         for i, (off, rows, cols) in enumerate(matrices):
-            r, c, rp, cp, tall, parts, chunk, sx, need, is_small = shapes[i]
-            mats[i] = (off, off, cols, cols, floats, rows, cols, r, c, rp, cp, tall, parts, chunk, sx, math.sqrt(max(1.0, cols / rows)), 0)
+            r, c, rp, cp, tall, parts, chunk, need, is_small = shapes[i]
+            mats[i] = (off, off, cols, cols, floats, rows, cols, r, c, rp, cp, tall, parts, chunk, math.sqrt(max(1.0, cols / rows)))
             floats += (need + 63) // 64 * 64
             flat += [(i, k) for k in range(parts)]
             blocks = [(i, k) for k in range((rp // 32) * (cp // 32))]
