@@ -532,15 +532,16 @@ PYBIND11_MODULE(_hip, m) {
       steps = (int)(v.size() / 3);
       for (int k = 0; k < steps; ++k) out[k] = NsCoeffs{v[3 * k], v[3 * k + 1], v[3 * k + 2]};
     };
-    m.def("newton_schulz_workspace", [](int kind, int batch, int rows, int cols) {
+    m.def("newton_schulz_workspace", [](int kind, int batch, int rows, int cols, bool fp32) {
       NsArgs a{};
-      a.kind = kind; a.batch = batch; a.rows = rows; a.cols = cols;
+      a.kind = kind; a.batch = batch; a.rows = rows; a.cols = cols; a.fp32 = fp32;
       return ns_workspace(a);
     });
     m.def("newton_schulz", [coeffs](int kind, int batch, int rows, int cols, uint64_t g, long long ld, long long g_stride, uint64_t out,
-                                    long long out_ld, long long out_stride, double eps, const std::vector<float>& co, float growth, uint64_t ws,
-                                    size_t ws_bytes, uint64_t stream) {
+                                    long long out_ld, long long out_stride, double eps, const std::vector<float>& co, float growth, bool fp32,
+                                    uint64_t ws, size_t ws_bytes, uint64_t stream) {
       NsArgs a{};
+      a.fp32 = fp32;
       a.kind = kind; a.batch = batch; a.rows = rows; a.cols = cols;
       a.g = reinterpret_cast<const void*>(g); a.ld = ld; a.g_stride = g_stride;
       a.out = reinterpret_cast<void*>(out); a.out_ld = out_ld; a.out_stride = out_stride;
@@ -567,7 +568,7 @@ PYBIND11_MODULE(_hip, m) {
       MuonArgs a{};
       P(p, float); P(g, const float); P(m, float); P(v, float); P(hyper, const float); P(mats, const NsMat);
       P(items_flat, const NsItem); P(items_small, const NsItem); P(items_split, const NsItem); P(items_gram, const NsItem); P(items_join, const NsItem); P(parts, float); P(items_sym, const NsItem); P(items_apply, const NsItem);
-      V(n_flat); V(n_small); V(n_out); V(n_split); V(n_gram); V(n_sym); V(n_apply); V(nesterov); V(eps); V(growth);
+      V(n_flat); V(n_small); V(n_out); V(n_split); V(n_gram); V(n_sym); V(n_apply); V(nesterov); V(eps); V(growth); V(fp32);
       coeffs(d["coeffs"].cast<std::vector<float>>(), a.coeffs, a.steps);
       muon_step(a, as_ptr<void>(d, "ws"), as_stream(stream));
     });

@@ -17,7 +17,7 @@ constexpr int kNsNormParts = 512;   // partial sums of a squared norm
 // One matrix. Its workspace (base `ws`, in floats from the call's workspace) holds
 //   [kNsNormParts doubles][tau, 63 spare][X, X': rp x cp pairs][A, P: rp x rp pairs]
 // with sides padded to multiples of 32 by zeros. A pair is two fp16 numbers h + l in 4 bytes, laid out per row in
-// blocks of 32: 32 h, then 32 l.
+// blocks of 32: 32 h, then 32 l. Products in fp32 keep fp32 numbers there instead, in the same 4 bytes.
 struct NsMat {
   long long src, out;   // element offset of G, and of the output / parameter
   long long ld, out_ld; // row strides
@@ -62,6 +62,7 @@ struct NsArgs {
   double eps;
   NsCoeffs coeffs[kNsMaxSteps];
   float growth;         // a power of two that bounds |a + b s + c s^2| over the values that s takes
+  int fp32;             // products of fp32 numbers instead of pairs
 };
 size_t ns_workspace(const NsArgs& a);
 void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t stream);
@@ -87,6 +88,7 @@ struct MuonArgs {
   double eps;
   NsCoeffs coeffs[kNsMaxSteps];
   float growth;
+  int fp32;                                 // products of fp32 numbers; the tables then hold no small matrices
 };
 constexpr int kMuonTile = 64;
 constexpr int kMuonVecChunk = 1024;   // vector elements per item

@@ -5,10 +5,13 @@
 // measures what fp32 products leave, in the norm of the whole (1e-6 - 1e-5 relative, 64x10 to 1024x2048). Everything is kept times the largest
 // power of two that fits fp16: X by 2^13, A and P by 2^12. An element keeps its 22 bits down to 2^-16 (X) and 2^-15; below, the pair's smallest step is
 // a floor: 2^-38 and 2^-37 at most. Rows or columns far below the others feel it, and fp32 products would not (64 x 256, one row scaled by 1e-2 / 1e-4 / 1e-6:
-// its relative error 2e-7 / 3e-6 / 3e-4, by fp32 products 3e-7).
+// its relative error 4e-7 / 3e-6 / 2e-4, by fp32 products 4e-7; 1024 x 4096 1e-6 / 4e-5 / 5e-3, by fp32 products 2e-6).
 // A matrix whose norm is far below eps starts with tiny X_0; its part below one is carried apart in tau (a power of two per
 // matrix, grown by `growth` per step up to 1), so that the fp16 numbers never see it: X = tau Xs,
 //   Xs <- (tau / tau') (a I + b tau^2 As + c tau^4 As^2) Xs.
+//
+// A caller to whom such rows matter takes products of fp32 numbers (NsArgs::fp32) instead: the same kernels on the fp32 matrix pipe, by tiles for
+// every size (us of a call by pairs / fp32 numbers: 6 x 576 x 64 68 / 125, 1024 x 1024 209 / 365, 4096 x 4096 3365 / 10974).
 //
 // A step is three products: A = X X^T and P = a I + b A + c A^2 are symmetric, so only the tiles on and below the diagonal are
 // computed and each is stored twice; X' = P X. The last one writes the output (or updates the parameter) directly.
@@ -38,6 +41,7 @@ struct NsDev {
   int step, last;
   float growth;
   NsCoeffs co;
+  int fp32;                    // fp32 numbers in place of pairs
   int splits;                  // parts of a tile of X X^T, table == nullptr
   float* parts;                // their sums, as the accumulators lie in the registers of a workgroup
 };
@@ -193,6 +197,18 @@ __device__ __forceinline__ floatx4 pair_load4(const float* base, int pitch, int 
   return __builtin_convertvector(*reinterpret_cast<const halfx4*>(p), floatx4) + __builtin_convertvector(*reinterpret_cast<const halfx4*>(p + 64), floatx4);
 }
 
+// Four values of X, A or P as the products read them: pairs, or fp32 numbers in their place
+template <MmKind KIND>
+__device__ __forceinline__ void ns_store4(float* base, int pitch, int row, int col, const floatx4& v) {
+  if constexpr (KIND == MM_F32) *reinterpret_cast<floatx4*>(base + (long long)row * pitch + col) = v;
+  else pair_store4(base, pitch, row, col, v);
+}
+template <MmKind KIND>
+__device__ __forceinline__ floatx4 ns_load4(const float* base, int pitch, int row, int col) {
+  if constexpr (KIND == MM_F32) return *reinterpret_cast<const floatx4*>(base + (long long)row * pitch + col);
+  else return pair_load4(base, pitch, row, col);
+}
+
 // G / (|G| + eps) / tau as pairs, one 32 x 32 block of X per workgroup (transposed on the way where G is tall).
 __global__ __launch_bounds__(256) void ns_split_kernel(NsDev a) {
   __shared__ double scratch[4];
@@ -230,7 +246,9 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsDev a) {
   }
   __syncthreads();
   const int y = threadIdx.x >> 3, x = (threadIdx.x & 7) * 4;
-  pair_store4(a.ws + ns_x(m), m.cp, bi * 32 + y, bj * 32 + x, floatx4{block[y][x], block[y][x + 1], block[y][x + 2], block[y][x + 3]});
+  const floatx4 v = {block[y][x], block[y][x + 1], block[y][x + 2], block[y][x + 3]};
+  if (a.fp32) ns_store4<MM_F32>(a.ws + ns_x(m), m.cp, bi * 32 + y, bj * 32 + x, v);
+  else ns_store4<MM_PAIR>(a.ws + ns_x(m), m.cp, bi * 32 + y, bj * 32 + x, v);
 }
 
 // Element (row, col) of the output, or of the parameter that it updates.
@@ -261,11 +279,11 @@ struct NsTile {
   static constexpr NsTileInfo I = kNsTiles[T / 64 - 1];
   static constexpr int WGM = I.wgm, WGN = I.wgn, STAGES = I.stages, SUBS = I.subs, NT = 64 * WGM * WGN;
 };
-template <int T, bool KCB, bool SWAP>
-using NsLoop = MmDirect<MM_PAIR, true, KCB, T, T, NsTile<T>::WGM, NsTile<T>::WGN, SWAP, NsTile<T>::STAGES, NsTile<T>::SUBS>;
+template <MmKind KIND, int T, bool KCB, bool SWAP>
+using NsLoop = MmDirect<KIND, true, KCB, T, T, NsTile<T>::WGM, NsTile<T>::WGN, SWAP, NsTile<T>::STAGES, NsTile<T>::SUBS>;
 
 // One T x T tile of one of the three products.
-template <NsOp OP, int T>
+template <MmKind KIND, NsOp OP, int T>
 __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
   extern __shared__ __attribute__((aligned(16))) char ns_smem[];
   const int t = mm_item(blockIdx.x, a.total);
@@ -327,7 +345,7 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
       const int pitch = GRAM ? m.cp : m.rp;
       const char* s = reinterpret_cast<const char*>(GRAM ? xa : A);
       const int kb = OP == NS_GRAM_PART ? k0 * 32 : 0, ke = OP == NS_GRAM_PART ? (k0 + kn) * 32 : pitch;
-      NsLoop<T, true, true>::run(MmOperands{s, s, pitch, pitch, m.rp, m.rp}, m0, n0, kb, ke, ns_smem, acc);
+      NsLoop<KIND, T, true, true>::run(MmOperands{s, s, pitch, pitch, m.rp, m.rp}, m0, n0, kb, ke, ns_smem, acc);
     }
     if constexpr (OP == NS_GRAM_PART) {
       floatx4* d = reinterpret_cast<floatx4*>(a.parts) + slot * (MI * NJ * NsTile<T>::NT) + threadIdx.x;
@@ -358,13 +376,18 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
         if (nn >= m.rp) continue;
         floatx4 v = acc[i][j] * cc;
         if (OP == NS_POLY) {
-          v += pair_load4(A, m.rp, mm, nn) * cb;
+          v += ns_load4<KIND>(A, m.rp, mm, nn) * cb;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (mm == nn + e && mm < m.r) v[e] += ca;
         }
-        pair_store4(dst, m.rp, mm, nn, v);
-        if (m0 != n0) {   // the mirrored tile
+        ns_store4<KIND>(dst, m.rp, mm, nn, v);
+        if (m0 == n0) continue;
+        // the mirrored tile
+        if constexpr (KIND == MM_F32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dst[(long long)(nn + e) * m.rp + mm] = v[e];
+        } else {
           halfx4 h, l;
           pair_split(v, h, l);
 #pragma unroll
@@ -380,8 +403,8 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
   }
 
   const MmOperands o{reinterpret_cast<const char*>(P), reinterpret_cast<const char*>(xa), m.rp, m.cp, m.rp, m.cp};
-  if (!a.last || !m.tall) NsLoop<T, false, true>::run(o, m0, n0, 0, m.rp, ns_smem, acc);
-  else NsLoop<T, false, false>::run(o, m0, n0, 0, m.rp, ns_smem, acc);
+  if (!a.last || !m.tall) NsLoop<KIND, T, false, true>::run(o, m0, n0, 0, m.rp, ns_smem, acc);
+  else NsLoop<KIND, T, false, false>::run(o, m0, n0, 0, m.rp, ns_smem, acc);
   if (!a.last) {
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -389,7 +412,7 @@ __global__ __launch_bounds__(NsTile<T>::NT) void ns_product_kernel(NsDev a) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int nn = n0 + wn + j * 16 + 4 * q;
-        if (mm < m.rp && nn < m.cp) pair_store4(xb, m.cp, mm, nn, acc[i][j] * (1.f / kScaleP));
+        if (mm < m.rp && nn < m.cp) ns_store4<KIND>(xb, m.cp, mm, nn, acc[i][j] * (1.f / kScaleP));
       }
     }
     return;
@@ -657,25 +680,34 @@ __global__ __launch_bounds__(256) void ns_out_kernel(NsDev a) {
   }
 }
 
-void gram_in_parts(const char* part, const char* join, const NsDev& p, const NsDev& j, hipStream_t stream) {
+template <MmKind KIND>
+void gram_in_parts_as(const char* part, const char* join, const NsDev& p, const NsDev& j, hipStream_t stream) {
   constexpr int T = kNsSplitTile;
-  const size_t lds = NsLoop<T, true, true>::LDS;
-  launch(part, ns_product_kernel<NS_GRAM_PART, T>, dim3((unsigned)((p.total + 7) / 8 * 8)), dim3(NsTile<T>::NT), lds, stream, p);
-  launch(join, ns_product_kernel<NS_GRAM_JOIN, T>, dim3((unsigned)((j.total + 7) / 8 * 8)), dim3(NsTile<T>::NT), 0, stream, j);
+  const size_t lds = NsLoop<KIND, T, true, true>::LDS;
+  launch(part, ns_product_kernel<KIND, NS_GRAM_PART, T>, dim3((unsigned)((p.total + 7) / 8 * 8)), dim3(NsTile<T>::NT), lds, stream, p);
+  launch(join, ns_product_kernel<KIND, NS_GRAM_JOIN, T>, dim3((unsigned)((j.total + 7) / 8 * 8)), dim3(NsTile<T>::NT), 0, stream, j);
+}
+void gram_in_parts(const char* part, const char* join, const NsDev& p, const NsDev& j, hipStream_t stream) {
+  if (p.fp32) gram_in_parts_as<MM_F32>(part, join, p, j, stream);
+  else gram_in_parts_as<MM_PAIR>(part, join, p, j, stream);
 }
 template <NsOp OP>
 void product(const char* name, NsDev d, int tile, hipStream_t stream) {
-  const dim3 grid((unsigned)((d.total + 7) / 8 * 8));
-  if (tile == 256) launch(name, ns_product_kernel<OP, 256>, grid, dim3(512), NsLoop<256, true, true>::LDS, stream, d);
-  else if (tile == 192) launch(name, ns_product_kernel<OP, 192>, grid, dim3(512), NsLoop<192, true, true>::LDS, stream, d);
-  else if (tile == 128) launch(name, ns_product_kernel<OP, 128>, grid, dim3(NsTile<128>::NT), NsLoop<128, true, true>::LDS, stream, d);
-  else launch(name, ns_product_kernel<OP, 64>, grid, dim3(NsTile<64>::NT), NsLoop<64, true, true>::LDS, stream, d);
+  auto as = [&](auto kernel, int threads, size_t lds) { launch(name, kernel, dim3((unsigned)((d.total + 7) / 8 * 8)), dim3(threads), lds, stream, d); };
+  if (d.fp32) as(ns_product_kernel<MM_F32, OP, 64>, NsTile<64>::NT, NsLoop<MM_F32, 64, true, true>::LDS);
+  else if (tile == 256) as(ns_product_kernel<MM_PAIR, OP, 256>, 512, NsLoop<MM_PAIR, 256, true, true>::LDS);
+  else if (tile == 192) as(ns_product_kernel<MM_PAIR, OP, 192>, 512, NsLoop<MM_PAIR, 192, true, true>::LDS);
+  else if (tile == 128) as(ns_product_kernel<MM_PAIR, OP, 128>, NsTile<128>::NT, NsLoop<MM_PAIR, 128, true, true>::LDS);
+  else as(ns_product_kernel<MM_PAIR, OP, 64>, NsTile<64>::NT, NsLoop<MM_PAIR, 64, true, true>::LDS);
 }
 
 int sym_tiles(const NsMat& m, int T) { const int t = ceil_div(m.rp, T); return t * (t + 1) / 2; }
 // The tile with the least estimated time: rounds of workgroups times k.
 template <class Count>
-int pick_tile(Count&& count, int k_stages) {
+int pick_tile(Count&& count, int k_stages, int fp32) {
+  // fp32 numbers: 64 x 64 for every size (us of a call of five steps by 64 / 128: 512 x 512 214 / 537, 1024 x 4096 745 / 1858, 2048 x 2048 1717 / 1878,
+  // 4096 x 4096 10974 / 11984; 128 for P X of the last two alone would gain 0 and 4 %)
+  if (fp32) return 64;
   int best = 64;
   float least = 0.f;
   for (const NsTileInfo& i : kNsTiles) {
@@ -707,9 +739,9 @@ void ns_shape(NsMat& m, int rows, int cols) {
 
 namespace {
 // parts of X X^T of a uniform call, 1 where a tile kernel does it alone
-int gram_splits(const NsMat& m, int batch) {
+int gram_splits(const NsMat& m, int batch, int fp32) {
   const long long tiles = (long long)sym_tiles(m, kNsSplitTile) * batch;
-  if (ns_small(m) || pick_tile([&](int T) { return (long long)sym_tiles(m, T) * batch; }, m.cp / 32) != kNsSplitTile) return 1;
+  if ((ns_small(m) && !fp32) || pick_tile([&](int T) { return (long long)sym_tiles(m, T) * batch; }, m.cp / 32, fp32) != kNsSplitTile) return 1;
   return ns_splits(m, tiles);
 }
 }  // namespace
@@ -717,7 +749,7 @@ int gram_splits(const NsMat& m, int batch) {
 size_t ns_workspace(const NsArgs& a) {
   NsMat m{};
   ns_shape(m, a.rows, a.cols);
-  const int s = gram_splits(m, a.batch);
+  const int s = gram_splits(m, a.batch, a.fp32);
   const long long parts = s > 1 ? (long long)sym_tiles(m, kNsSplitTile) * a.batch * s * kNsSplitTile * kNsSplitTile : 0;
   return (size_t)(ns_floats(m) * a.batch + parts) * sizeof(float);
 }
@@ -732,7 +764,7 @@ void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t strea
   d.g = a.g; d.out = a.out; d.kind = a.kind;
   d.g_stride = a.g_stride; d.out_stride = a.out_stride; d.ws_stride = ns_floats(d.one);
   d.ws = reinterpret_cast<float*>(ws);
-  d.eps = a.eps; d.growth = a.growth;
+  d.eps = a.eps; d.growth = a.growth; d.fp32 = a.fp32;
   const NsMat& m = d.one;
   auto with = [&](int per) {
     if ((long long)per * a.batch > 0x7ffff8) throw std::runtime_error("newton_schulz: too many tiles");   // x 512 threads: below 2^32
@@ -745,7 +777,7 @@ void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t strea
   launch("ns_norm", ns_norm_kernel, dim3(n.total), dim3(256), 0, stream, n);
   const NsDev s = with((m.rp / 32) * (m.cp / 32));
   launch("ns_split", ns_split_kernel, dim3(s.total), dim3(256), 0, stream, s);
-  if (ns_small(m)) {
+  if (ns_small(m) && !a.fp32) {
     NsSmallArgs k{};
     k.d = with(1);
     k.steps = a.steps;
@@ -755,12 +787,12 @@ void newton_schulz(const NsArgs& a, void* ws, size_t ws_bytes, hipStream_t strea
     return;
   }
   // X X^T of few rows and many columns: in parts, which are added in order (us of 512 x 3136 26 -> 15, of 1024 x 4096 36 -> 26)
-  const int splits = gram_splits(m, a.batch);
+  const int splits = gram_splits(m, a.batch, a.fp32);
   d.splits = splits;
   d.parts = d.ws + ns_floats(m) * a.batch;
-  const int tg = pick_tile([&](int T) { return (long long)sym_tiles(m, T) * a.batch; }, m.cp / 32);
-  const int tp = pick_tile([&](int T) { return (long long)sym_tiles(m, T) * a.batch; }, m.rp / 32);
-  const int ta = pick_tile([&](int T) { return (long long)apply_tiles(m, T) * a.batch; }, m.rp / 32);
+  const int tg = pick_tile([&](int T) { return (long long)sym_tiles(m, T) * a.batch; }, m.cp / 32, a.fp32);
+  const int tp = pick_tile([&](int T) { return (long long)sym_tiles(m, T) * a.batch; }, m.rp / 32, a.fp32);
+  const int ta = pick_tile([&](int T) { return (long long)apply_tiles(m, T) * a.batch; }, m.rp / 32, a.fp32);
   for (int k = 0; k < a.steps; ++k) {
     d.step = k;
     d.last = k == a.steps - 1;
@@ -783,7 +815,7 @@ void muon_step(const MuonArgs& a, void* ws, hipStream_t stream) {
   d.table = a.mats;
   d.ws = reinterpret_cast<float*>(ws);
   d.g = a.g; d.out = a.p; d.m = a.m; d.v = a.v; d.hyper = a.hyper; d.kind = MM_F32;
-  d.nesterov = a.nesterov; d.eps = a.eps; d.growth = a.growth; d.parts = a.parts;
+  d.nesterov = a.nesterov; d.eps = a.eps; d.growth = a.growth; d.parts = a.parts; d.fp32 = a.fp32;
   auto with = [&](const NsItem* items, int total) {
     NsDev x = d;
     x.items = items;

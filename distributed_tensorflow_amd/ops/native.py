@@ -1264,16 +1264,28 @@ def _ns_steps(coeffs: tuple, steps: int) -> tuple:
     return flat, 2.0 ** math.ceil(math.log2(factor))
 
 
+PRODUCTS = ("pairs", "fp32")
+
+
+def _ns_fp32(products: str) -> bool:
+    if products not in PRODUCTS:
+        raise ValueError(f"newton_schulz: products are {' or '.join(PRODUCTS)}, got {products!r}")
+    return products == "fp32"
+
+
 def _ns_key(coeffs) -> tuple:
     return tuple(tuple(float(v) for v in c) for c in coeffs) if isinstance(coeffs[0], (tuple, list)) else tuple(float(v) for v in coeffs)
 
 
-def newton_schulz(g, *, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out=None, workspace=None):
+def newton_schulz(g, *, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, products: str = "pairs", out=None, workspace=None):
     """Orthogonalises the matrix g [m,n], or every matrix of g [batch,m,n], by Newton-Schulz steps
     (csrc/kernels/newton_schulz.hip): X = g / (|g| + eps), then X <- a X + (b A + c A^2) X with A = X X^T.
 
-    float32, bfloat16 or float16 in and out; the products run on fp16 pairs (22 bits) with fp32 sums whatever the
-    type, since five steps amplify an early rounding error up to 485-fold. Rows may be strided. coeffs: (a, b, c), or
+    float32, bfloat16 or float16 in and out, fp32 sums. Five steps amplify an early rounding error up to 485-fold, so the
+    products need more than 16 bits whatever the type. products="pairs" multiplies pairs of fp16 numbers: 22 bits of
+    every element down to 2^-16 of |X| = 1, and the accuracy of fp32 products in the norm of the result, but not in rows or
+    columns far below the others (a row scaled by 1e-4 / 1e-8: off by 3e-6 / 3e-2 of its size in 64 x 256, 4e-5 / 4e-1 in
+    1024 x 4096). products="fp32" multiplies fp32 numbers, which keeps such rows, in 1.5 to 3.3 times the time. Rows may be strided. coeffs: (a, b, c), or
     a triple for every step; sequences whose iterates would leave the pairs' range are refused. out may be g itself.
     workspace: newton_schulz_workspace() bytes; a call recorded into a step program has to bring its own."""
     _check_no_grad("newton_schulz", g)
@@ -1282,6 +1294,7 @@ def newton_schulz(g, *, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out
     if not eps > 0:
         raise ValueError("newton_schulz: eps must be positive")
     flat, growth = _ns_steps(_ns_key(coeffs), steps)
+    fp32 = _ns_fp32(products)
     rows, cols = g.shape[-2:]
 
     def place(t, what, written):
@@ -1302,31 +1315,35 @@ def newton_schulz(g, *, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7, out
         return out
     batch = g.shape[0] if g.dim() == 3 else 1
     kind = _KINDS[g.dtype]
-    need = _hip.newton_schulz_workspace(kind, batch, rows, cols)
+    need = _hip.newton_schulz_workspace(kind, batch, rows, cols, fp32)
     ws, addr, have = _workspace("newton_schulz", need, workspace, g.device, (g, out))
-    _hip.newton_schulz(kind, batch, rows, cols, *pg, *po, eps, flat, growth, addr, have, _raw_stream(dev))
+    _hip.newton_schulz(kind, batch, rows, cols, *pg, *po, eps, flat, growth, fp32, addr, have, _raw_stream(dev))
     return out
 
 
-def newton_schulz_workspace(m: int, n: int, batch: int = 1) -> int:
+def newton_schulz_workspace(m: int, n: int, batch: int = 1, products: str = "pairs") -> int:
     """Bytes of workspace that newton_schulz() needs for [batch, m, n]."""
-    return hip().newton_schulz_workspace(0, batch, m, n)
+    return hip().newton_schulz_workspace(0, batch, m, n, _ns_fp32(products))
 
 
 class MuonTables:
     """What one optimizer's muon_step launches work from: the matrices of a flat parameter buffer, the work items of every
-    launch and the workspace, on the device. `matrices`: (offset, rows, cols); `vectors`: (offset, elements)."""
+    launch and the workspace, on the device. `matrices`: (offset, rows, cols); `vectors`: (offset, elements);
+    `products` as in newton_schulz."""
 
     MAT = np.dtype([("src", "<i8"), ("out", "<i8"), ("ld", "<i8"), ("out_ld", "<i8"), ("ws", "<i8"), ("rows", "<i4"), ("cols", "<i4"), ("r", "<i4"),
                     ("c", "<i4"), ("rp", "<i4"), ("cp", "<i4"), ("tall", "<i4"), ("parts", "<i4"), ("chunk", "<i4"), ("scale", "<f4")])
 
-    def __init__(self, matrices, vectors, device):
+    def __init__(self, matrices, vectors, device, products: str = "pairs"):
         require()
         h = hip()
+        self.fp32 = _ns_fp32(products)
         assert self.MAT.itemsize == h.NS_MAT_BYTES and h.NS_ITEM_BYTES == 24
         mats = np.zeros(len(matrices), dtype=self.MAT)
         flat, small, out, split, gram, join, sym, apply, floats, tile = [], [], [], [], [], [], [], [], 0, h.MUON_TILE
         shapes = [h.ns_shape(rows, cols) for _, rows, cols in matrices]
+        if self.fp32:   # every size by tiles
+            shapes = [s[:8] + (False,) for s in shapes]
         tiles_of = [0 if s[8] else (lambda t: t * (t + 1) // 2)(-(-s[2] // tile)) for s in shapes]   # of X X^T, lower triangle
         for i, (off, rows, cols) in enumerate(matrices):
             r, c, rp, cp, tall, parts, chunk, need, is_small = shapes[i]
@@ -1362,7 +1379,7 @@ class MuonTables:
         self._out = len(out)
 
     def launch_args(self) -> dict:
-        d = dict(mats=self._mats.data_ptr(), ws=self.workspace.data_ptr(), parts=self.workspace.data_ptr() + 4 * self._parts, n_out=self._out)
+        d = dict(mats=self._mats.data_ptr(), ws=self.workspace.data_ptr(), parts=self.workspace.data_ptr() + 4 * self._parts, n_out=self._out, fp32=int(self.fp32))
         for name, t in self._items.items():
             d["items_" + name], d["n_" + name] = t.data_ptr(), t.shape[0]
         return d

@@ -104,6 +104,9 @@ class FlatMuon(_FlatOptimizer):
     decoupled weight decay. Everything else (biases, normalisation parameters, and matrices not named in `matrices`)
     is updated by Adam with `vector_lr`. Slot "m" holds the momentum of either kind, "v" the vectors' second moments.
 
+    ns_products: what the orthogonalisation multiplies, "pairs" or "fp32" as in ops/native.py::newton_schulz; a CPU arena is
+    updated in fp32 either way.
+
     On a GPU a step is 2 + 3 * ns_steps launches whatever the number of parameters: every launch works on all
     matrices at once from tables built here."""
 
@@ -111,10 +114,12 @@ class FlatMuon(_FlatOptimizer):
 
     def __init__(self, arena: ParamArena, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, ns_steps: int = 5,
                  ns_coeffs=ref.NS_COEFFS, ns_eps: float = 1e-7, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
-                 matrices: Optional[Iterable[str]] = None):
+                 matrices: Optional[Iterable[str]] = None, ns_products: str = "pairs"):
         super().__init__(arena)
         if not ns_eps > 0:
             raise ValueError("FlatMuon: ns_eps must be positive")   # a matrix without a gradient would be 0 / 0
+        if ns_products not in ("pairs", "fp32"):
+            raise ValueError(f"FlatMuon: ns_products is 'pairs' or 'fp32', got {ns_products!r}")
         self.momentum, self.nesterov, self.weight_decay = momentum, nesterov, weight_decay
         self.ns_steps, self.ns_coeffs, self.ns_eps = ns_steps, ns_coeffs, ns_eps
         self.beta1, self.beta2, self.eps = beta1, beta2, eps
@@ -135,7 +140,7 @@ class FlatMuon(_FlatOptimizer):
                 self._vectors.append((off, s.numel))
         if self._gpu:
             self._nv._ns_steps(self._nv._ns_key(ns_coeffs), ns_steps)   # refuses coefficients here rather than in the first step
-            self._tables = self._nv.MuonTables(self._matrices, self._vectors, arena.params.device)
+            self._tables = self._nv.MuonTables(self._matrices, self._vectors, arena.params.device, ns_products)
 
     def step(self, lr: float, grad_scale: float = 1.0, vector_lr: Optional[float] = None) -> None:
         """Updates every parameter from grads * grad_scale; vectors with step size `vector_lr` (default: lr)."""
