@@ -6,7 +6,7 @@ persistent loop the reload queues behind the next tile's prefetch and waits for 
 64-channel split forward kernel lost a quarter of its time that way). The check compiles each kernel
 file with -Rpass-analysis=kernel-resource-usage and reports every kernel above its allowance.
 
-    python tools/check_spills.py [file.hip ...]     (default: the kernels of the training steps)
+    python tools/check_spills.py [file.hip ...]     (default: the kernels of the training steps, of the dense layers and of Newton-Schulz)
 
 Exit status 1 if a kernel spills more registers than ALLOWED grants it (default 0).
 """
@@ -25,11 +25,15 @@ ROOT = Path(__file__).resolve().parent.parent
 STEP_FILES = ("conv_fprop_band.hip", "conv_bwd_fused.hip", "conv_fprop_split.hip", "conv_bwd_split.hip", "conv_bwd_split_pc.hip",
               "conv_wgrad_band.hip", "conv_dgrad_s2.hip", "conv_stem.hip", "conv5x5_tile.hip", "conv5x5_split.hip", "lenet_conv1.hip",
               "gemm.hip", "optim.hip", "bn.hip", "head.hip", "fc_head.hip", "elementwise.hip", "conv_wgrad.hip")
+# dense layers of any type, Newton-Schulz and the optimizer on it
+DENSE_FILES = ("linear.hip", "linear_f32.hip", "linear_bf16.hip", "linear_f16.hip", "newton_schulz.hip")
 # substring of the mangled kernel name -> spilled registers tolerated
 ALLOWED = {
     "conv_fprop_split_kernelILi64ELi8ELi8ELb0E": 2,    # two reloads per tile, outside the MFMA loop
     "conv_fprop_split_kernelILi64ELi8ELi8ELb1E": 32,   # data gradient as a forward product: not launched by the fused backward step
     "conv_bwd_split_kernelILi16ELi32ELi8ELb1ELi0ELb0E": 3,
+    "linear_tile_kernelILNS_6MmKindE0ENS_8MmDirectILS1_0ELb0ELb0ELi256E": 5,   # fp32 weight gradients by 256 x 256 tiles: around the main loop, not in it
+    "ns_small_kernel": 16,   # one kernel for seven sizes, with the registers of 64 x 768
     "conv_bwd_split_kernelILi16ELi32ELi8ELb1ELi0ELb1E": 8,   # the instrumented instantiation of bench/diag/split_bwd_timeline.py
 }
 
@@ -53,7 +57,7 @@ def spills(src: Path) -> list[tuple[str, int]]:
 
 
 def main(argv: list[str]) -> int:
-    files = [Path(a) for a in argv] or [ROOT / "csrc" / "kernels" / f for f in STEP_FILES if (ROOT / "csrc" / "kernels" / f).exists()]
+    files = [Path(a) for a in argv] or [ROOT / "csrc" / "kernels" / f for f in STEP_FILES + DENSE_FILES if (ROOT / "csrc" / "kernels" / f).exists()]
     with ThreadPoolExecutor(max_workers=min(6, len(files))) as ex:
         results = list(ex.map(spills, files))
     bad = kernels = 0
