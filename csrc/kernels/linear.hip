@@ -12,6 +12,7 @@ namespace {
 
 // Rows that the few-rows kernels take; more go through 32 x 64 tiles. 4096 x 4096, us by rows kernel / tiles: bf16 W [K,N] 1 row 10.6 / 9.7 (1024 x 1024
 // 5.2 / 6.5), 2 rows 12.0 / 9.9; W [N,K] 2 rows 8.6 / 9.9, 3 rows 10.6 / 9.9; fp32 W [K,N] 4 rows 16.6 / 20.1, 5 rows 18.7 / 20.2 (1024 x 1024 10.8 / 8.5).
+// One 16-bit row over W [K,N] thus goes by the small weight: the large one would be 0.9 us sooner by tiles.
 int lin_rows_max(const MmProduct& p) { return p.kind == MM_F32 ? 4 : p.kc_b ? 2 : 1; }
 constexpr size_t kMaxPartialBytes = 256ull << 20;   // partial sums of a split product
 
@@ -36,9 +37,9 @@ struct Plan {
 };
 // The larger the tile the less is loaded per product, but it takes about a tile per CU to use the card; and k in parts fills it with fewer
 // tiles, for the price of the parts' way through memory and a second launch. The choice goes by an estimate of the time: what a
-// workgroup takes for a stage of 128 bytes of k, alone on its CU and with as many as fit, and what a launch takes besides, in us (fitted
-// to 1700 products of 9 to 8192 rows and columns, which it gives within 5 % (fp32) and 10 %; what it picks takes 1.6 % more than the best of
-// them, and 14 % less than tiles picked first and parts of at least twelve stages after).
+// workgroup takes for a stage of 128 bytes of k, alone on its CU and with as many as fit, and what a launch takes besides, in us: a fit to times of every
+// tile and number of parts over sizes of 9 to 8192 (bench/linear_sweep.py times what it picks against the library's product: 0.84 of its time
+// in the geometric mean over 110 sizes, 0.78 of aligned ones).
 struct TileCost { int variant, per_cu; float alone, full, launch; };
 constexpr TileCost kTileCosts[2][4] = {
     {{LIN_64, 2, 0.58f, 1.11f, 4.7f}, {LIN_128, 1, 1.8f, 1.87f, 5.9f}, {LIN_256, 1, 7.0f, 7.0f, 11.3f}, {LIN_32, 3, 0.33f, 0.89f, 4.4f}},   // fp32

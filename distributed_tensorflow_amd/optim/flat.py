@@ -107,8 +107,11 @@ class FlatMuon(_FlatOptimizer):
     ns_products: what the orthogonalisation multiplies, "pairs" or "fp32" as in ops/native.py::newton_schulz; a CPU arena is
     updated in fp32 either way.
 
-    On a GPU a step is 2 + 3 * ns_steps launches whatever the number of parameters: every launch works on all
-    matrices at once from tables built here."""
+    On a GPU the launches of a step do not grow with the number of parameters, since every one works on all matrices at once from tables
+    built here: three (the scalars, momentum with the vectors' Adam, the matrices' split), two more for matrices of up to 64 x 768,
+    32 x 1024 or 16 x 2048, which one workgroup takes, and 4 * ns_steps for larger ones. The tables' workspace holds the iterates of all matrices
+    at once: 8 bytes per element of a long matrix, 18 of a square one (a whole ResNet-20 10, the MNIST network 12), next to
+    parameter, gradient and slots."""
 
     slots = ("m", "v")
 
@@ -143,7 +146,8 @@ class FlatMuon(_FlatOptimizer):
             self._tables = self._nv.MuonTables(self._matrices, self._vectors, arena.params.device, ns_products)
 
     def step(self, lr: float, grad_scale: float = 1.0, vector_lr: Optional[float] = None) -> None:
-        """Updates every parameter from grads * grad_scale; vectors with step size `vector_lr` (default: lr)."""
+        """Updates every parameter from grads * grad_scale. `vector_lr` is the vectors' Adam step size; it defaults to lr, which suits the
+        matrices (0.02 or so) and is ten times what Adam usually takes."""
         a, t = self.arena, self.steps + 1
         lr_t = (lr if vector_lr is None else vector_lr) * math.sqrt(1.0 - self.beta2 ** t) / (1.0 - self.beta1 ** t)
         if self._gpu:
