@@ -397,7 +397,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void linear_row_k_kernel(LinTileArg
   }
 }
 
-// dz = dy act'(pre) and the sums of its columns. A block takes 256 columns (four per thread) and rows_per_block
+// dz = dy act'(pre) and the sums of its columns. dz is rounded to the tensors' type, which is what the matrix pipe multiplies: dx and dW of 16-bit tensors are off by
+// 1.4 times their own rounding (8192 x 4096 x 4096 bf16 2.3e-3 of 64 bits, with dz in fp32 1.7e-3); the column sums take the unrounded values. A block takes 256 columns (four per thread) and rows_per_block
 // rows, a quarter of them per wave; the waves' sums are added in wave order, the blocks' by lin_colsum_kernel.
 struct LinDzArgs {
   const void* dy; long long lddy;
