@@ -121,8 +121,10 @@ class FlatMuon(_FlatOptimizer):
         super().__init__(arena)
         if not ns_eps > 0:
             raise ValueError("FlatMuon: ns_eps must be positive")   # a matrix without a gradient would be 0 / 0
-        if ns_products not in ("pairs", "fp32"):
-            raise ValueError(f"FlatMuon: ns_products is 'pairs' or 'fp32', got {ns_products!r}")
+        from ..ops import native as nv   # the same refusals on any device, and here rather than in the first step
+
+        nv._ns_steps(nv._ns_key(ns_coeffs), ns_steps)
+        nv._ns_fp32(ns_products)
         self.momentum, self.nesterov, self.weight_decay = momentum, nesterov, weight_decay
         self.ns_steps, self.ns_coeffs, self.ns_eps = ns_steps, ns_coeffs, ns_eps
         self.beta1, self.beta2, self.eps = beta1, beta2, eps
@@ -142,7 +144,6 @@ class FlatMuon(_FlatOptimizer):
             else:
                 self._vectors.append((off, s.numel))
         if self._gpu:
-            self._nv._ns_steps(self._nv._ns_key(ns_coeffs), ns_steps)   # refuses coefficients here rather than in the first step
             self._tables = self._nv.MuonTables(self._matrices, self._vectors, arena.params.device, ns_products)
 
     def step(self, lr: float, grad_scale: float = 1.0, vector_lr: Optional[float] = None) -> None:
