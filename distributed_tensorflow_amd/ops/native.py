@@ -1075,7 +1075,11 @@ def _check_device(t: torch.Tensor, what: str) -> int:
 
 
 def _check_no_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t is None or not t.requires_grad:
+            continue
         raise ValueError(f"{what}: autograd does not see this call, and a tensor requires a gradient: call it under torch.no_grad(), or detach")
 
 
